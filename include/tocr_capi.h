@@ -39,6 +39,9 @@ enum {
   TOCR_ERR_INJECTED = 5  /* forced by tocr_debug_inject_error (tests only)   */
 };
 
+/* ---- element types of the linear-layer entries --------------------------- */
+enum { TOCR_DTYPE_F16 = 0, TOCR_DTYPE_BF16 = 1, TOCR_DTYPE_F32 = 2 };
+
 /* Message of the last failing call on this thread ("" if none). */
 TOCR_API const char *tocr_last_error_string(void);
 /* Library version as 0xMMmmpp. */
@@ -121,6 +124,47 @@ TOCR_API int tocr_rec_head_ctc_f16(const void *d_feat, int batch_size, int seq_l
                                    int num_labels, int *d_tokens, int *d_lengths,
                                    float *d_line_scores, int *d_step_idx, float *d_step_prob,
                                    int *d_err, void *stream);
+
+/* ---- training and scoring of the recognizer's head ----------------------- */
+
+/* Cross entropy of the recognizer's linear head, logits never stored (no
+ * counterpart in the reference, which only serves):
+ *   l = feat W^T + bias,  lse[i] = log sum_j exp(l[i][j]),
+ *   loss[i] = lse[i] - l[i][target[i]].
+ * A target outside [0, num_classes) marks a padding row: its loss and lse are
+ * 0, it costs no product, and whatever its features hold (NaN too) reaches no
+ * output. The step indices that tocr_rec_head_ctc_f16 and the decoders write
+ * are targets as they are.
+ * d_feat [rows][K] and d_w [num_classes][K] row-major, both of `dtype`
+ * (TOCR_DTYPE_F16 or TOCR_DTYPE_BF16), 16-byte aligned; K a multiple of 8, 8
+ * to 256; d_bias fp32 [num_classes] or NULL (a -inf entry masks its class);
+ * d_targets int32, or int64 where targets_i64 is non-zero; rows up to 2^24.
+ * d_loss, d_lse fp32 [rows]. d_workspace: 256-byte aligned, of the size that
+ * tocr_rec_head_ce_workspace_bytes gives (0: sizes out of range); it is
+ * scratch of one call, so calls that may overlap need their own. d_err as in
+ * tocr_rec_head_ctc_f16. Same inputs, same bits. */
+TOCR_API size_t tocr_rec_head_ce_workspace_bytes(long long rows, int K, int num_classes,
+                                                 int backward);
+TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *d_bias,
+                              const void *d_targets, int targets_i64, long long rows, int K,
+                              int num_classes, int dtype, float *d_loss, float *d_lse,
+                              void *d_workspace, size_t workspace_bytes, int *d_err,
+                              void *stream);
+
+/* Its gradient for a weight g = d_grad_loss[i] of every row's loss, with
+ * d_lse as the forward call wrote it for the same inputs:
+ *   G[i][j] = g[i] (exp(l[i][j] - lse[i]) - [j = target[i]]),
+ *   dfeat = G W, dw = G^T feat, dbias[j] = sum_i G[i][j].
+ * d_dfeat [rows][K] and d_dw [num_classes][K] of `dtype`, d_dbias fp32; each
+ * may be NULL (not wanted). Outputs are overwritten, not added to; padding
+ * rows get zero gradients and their g and lse are not used. The workspace is
+ * that of backward = 1. Outputs must not overlap inputs. */
+TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, const float *d_bias,
+                                       const void *d_targets, int targets_i64, long long rows,
+                                       int K, int num_classes, int dtype, const float *d_lse,
+                                       const float *d_grad_loss, void *d_dfeat, void *d_dw,
+                                       float *d_dbias, void *d_workspace, size_t workspace_bytes,
+                                       int *d_err, void *stream);
 
 /* Allocation-free variant of tocr_ctc_greedy_f16 (no counterpart in the
  * reference). It is for callers that may not call cudaMalloc at all: plugins
