@@ -41,6 +41,7 @@ enum {
 
 /* ---- element types of the linear-layer entries --------------------------- */
 enum { TOCR_DTYPE_F16 = 0, TOCR_DTYPE_BF16 = 1, TOCR_DTYPE_F32 = 2 };
+enum { TOCR_ACT_NONE = 0, TOCR_ACT_RELU = 1, TOCR_ACT_HARDSWISH = 2 };
 
 /* Message of the last failing call on this thread ("" if none). */
 TOCR_API const char *tocr_last_error_string(void);
@@ -165,6 +166,39 @@ TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, cons
                                        const float *d_grad_loss, void *d_dfeat, void *d_dw,
                                        float *d_dbias, void *d_workspace, size_t workspace_bytes,
                                        int *d_err, void *stream);
+
+/* ---- INT8 linear layer ---------------------------------------------------- */
+
+/* Rows of INT8 codes with one fp32 scale each: of activations (a scale per
+ * token) or of a weight matrix [N][K] (a scale per output channel; lay it out
+ * once). The per-pixel / per-channel numerics of tocr_dwpw_block:
+ *   scale = max(max_k |x[k]| / 127, 2^-126) rounded to fp32,
+ *   code[k] = x[k] / scale to the nearest integer (ties to even).
+ * A row that holds an infinity or a NaN gets the scale NaN and codes 0.
+ * d_x [rows][K] of x_dtype (any TOCR_DTYPE_*, aligned to its element);
+ * d_codes int8 [rows][pitch], pitch = K rounded up to a multiple of 16, zero
+ * behind K, 16-byte aligned; d_scales [rows]. rows up to 2^24, K up to 2^17. */
+TOCR_API int tocr_quant_rows_i8(const void *d_x, int x_dtype, long long rows, int K, void *d_codes,
+                                float *d_scales, void *stream);
+
+/* y[m][n] = act(sx[m] sw[n] sum_k xq[m][k] wq[n][k] + bias[n]) on codes and
+ * scales as tocr_quant_rows_i8 lays them out (both pitches K rounded up to 16,
+ * zeros behind K). The sum is exact; the rest is fp32, rounded once to
+ * out_dtype. d_bias fp32 [N] or NULL; act TOCR_ACT_*; d_y [rows][N] of
+ * out_dtype, aligned to its element, any N; d_err as in
+ * tocr_rec_head_ctc_f16. */
+TOCR_API int tocr_linear_i8_codes(const void *d_xq, const float *d_sx, long long rows, int K,
+                                  const void *d_wq, const float *d_sw, const float *d_bias, int N,
+                                  int act, int out_dtype, void *d_y, int *d_err, void *stream);
+
+/* The layer on activations as they are: tocr_quant_rows_i8 of d_x into the
+ * workspace (256-byte aligned, tocr_linear_i8_workspace_bytes, scratch of one
+ * call), then tocr_linear_i8_codes. */
+TOCR_API size_t tocr_linear_i8_workspace_bytes(long long rows, int K);
+TOCR_API int tocr_linear_i8(const void *d_x, int x_dtype, long long rows, int K, const void *d_wq,
+                            const float *d_sw, const float *d_bias, int N, int act, int out_dtype,
+                            void *d_y, void *d_workspace, size_t workspace_bytes, int *d_err,
+                            void *stream);
 
 /* Allocation-free variant of tocr_ctc_greedy_f16 (no counterpart in the
  * reference). It is for callers that may not call cudaMalloc at all: plugins

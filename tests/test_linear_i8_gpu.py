@@ -1,0 +1,82 @@
+"""The INT8 linear layer (turboocr_b200.linear_i8) against its definition in 64
+bits. Codes and scales must be equal. The sum of the products of codes is
+exact; behind it come the conversion to fp32 (2^-24, exact below 2^24), two
+products, the bias and the activation in fp32 (each at most 2^-24 of the
+largest term: 8 * 2^-24 together) and one rounding to the output type (half a
+step of the value, or half of the least subnormal)."""
+import math
+
+import pytest
+import torch
+
+from turboocr_b200 import linear_i8
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def quantized(x):
+    """Codes (fp64) and fp32 scales by the definition. The fp64 quotient of two
+    fp32 numbers is a tie only where the exact one is: q + 1/2 and its
+    neighbours in reach differ by far more than 2^-45."""
+    x32 = x.float()
+    s = (x32.abs().amax(1).cpu().double() / 127).float().clamp_min(2.0 ** -126).to(x.device)
+    bad = ~torch.isfinite(x32).all(1)
+    q = torch.round(x32.double() / s.double()[:, None])
+    q[bad] = 0
+    s[bad] = math.nan
+    return q, s
+
+
+def act64(y, act):
+    if act == "relu":
+        return torch.where(y < 0, torch.zeros_like(y), y)
+    if act == "hardswish":
+        return y * (y + 3).clamp(0, 6) / 6
+    return y
+
+
+def check(x, w, bias, act, out, err):
+    K = x.shape[1]
+    wq, ws = linear_i8.quantize_rows(w)
+    q, s = quantized(w)
+    assert torch.equal(wq[:, :K].double(), q) and torch.equal(ws, s)
+    assert int(wq[:, K:].abs().sum()) == 0
+    xq, sx = linear_i8.quantize_rows(x)
+    qx, s2 = quantized(x)
+    assert torch.equal(xq[:, :K].double(), qx) and torch.equal(sx, s2)
+    assert int(xq[:, K:].abs().sum()) == 0
+    y = linear_i8.linear(x, wq, ws, bias, act=act, out_dtype=out, err=err)
+    y2 = linear_i8.linear_codes(xq, sx, K, wq, ws, bias, act=act, out_dtype=out, err=err)
+    torch.cuda.synchronize()
+    assert int(err) == 0
+    assert torch.equal(y, y2)
+    z = (qx @ q.T) * s2.double()[:, None] * s.double()
+    b = bias.double() if bias is not None else 0.0
+    want = act64(z + b, act)
+    # the activation's slope is at most 1.5; hardswish multiplies by up to |z + b|
+    mag = (z.abs() + (bias.abs().double() if bias is not None else 0.0)) * 1.5
+    u = torch.finfo(out).eps / 2
+    tiny = torch.finfo(out).smallest_normal * torch.finfo(out).eps / 2
+    tol = 8 * 2.0 ** -24 * mag + u * want.abs() + tiny
+    d = (y.double() - want).abs()
+    assert bool((d <= tol).all()), float((d / tol).max())
+    return y
+
+
+SIZES = [(1, 1, 1), (1, 512, 18385), (3, 17, 5), (80, 128, 384), (127, 100, 130), (129, 260, 255),
+         (128, 261, 64), (200, 1001, 257), (2560, 256, 1024), (5, 5000, 33), (1000, 64, 2049),
+         (257, 2048, 16), (33, 8200, 100)]
+
+
+@pytest.mark.parametrize("xt,yt", [(F16, F16), (BF16, BF16), (F32, F32), (F16, F32), (F32, BF16)])
+@pytest.mark.parametrize("rows,K,N", SIZES)
+def test_linear(tocr, cuda, rows, K, N, xt, yt):
+    g = torch.Generator(device="cpu").manual_seed(rows + 31 * K + 7 * N)
+    gain = torch.exp(torch.randn(K, generator=g))
+    x = (torch.randn(rows, K, generator=g) * gain).to(xt).to(cuda)
+    w = (torch.randn(N, K, generator=g) / math.sqrt(K)).to(cuda)
+    bias = torch.randn(N, generator=g).to(cuda) if (rows + N) % 2 else None
+    act = ["none", "relu", "hardswish"][(rows + K + N) % 3]
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    check(x, w, bias, act, yt, err)

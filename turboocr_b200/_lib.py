@@ -98,6 +98,11 @@ SIGNATURES: dict[str, tuple] = {
                               _vp, _vp]),
     "tocr_rec_head_ce_backward": (_i, [_vp, _vp, _vp, _vp, _i, _ll, _i, _i, _i, _vp, _vp, _vp,
                                        _vp, _vp, _vp, C.c_size_t, _vp, _vp]),
+    "tocr_quant_rows_i8": (_i, [_vp, _i, _ll, _i, _vp, _vp, _vp]),
+    "tocr_linear_i8_codes": (_i, [_vp, _vp, _ll, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "tocr_linear_i8_workspace_bytes": (C.c_size_t, [_ll, _i]),
+    "tocr_linear_i8": (_i, [_vp, _i, _ll, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, C.c_size_t,
+                            _vp, _vp]),
     "tocr_conv_tc_packed_bytes": (C.c_size_t, [_i, _i, _i]),
     "tocr_conv_tc_pack": (_i, [_i, _i, _i, _vp, _vp, C.c_size_t]),
     "tocr_conv_tc_f16": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
