@@ -50,26 +50,74 @@ __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 template <>
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// x / s to the nearest integer, ties to even, of the exact quotient: the
-// product with 1/s may miss a border by its rounding, so the remainder decides
-// (x - q s is exact in fp32 near half a step, both being on grids no finer than
-// s 2^-24).
-__device__ __forceinline__ int code_of(float x, float s, float inv) {
-  float q = rintf(x * inv);
-  const float r = fmaf(-q, s, x), h = 0.5f * s;
-  if (fabsf(r) >= h) {
-    const bool odd = (static_cast<int>(q) & 1) != 0;
-    if (r > h || (r == h && odd)) q += 1.f;
-    if (r < -h || (r == -h && odd)) q -= 1.f;
+// x / s to the nearest integer, ties to even, of the exact quotient. q is the
+// product with 1/s rounded by adding 1.5 * 2^23 (one fused step); the rounding
+// of 1/s can only miss next to a border, so where the remainder r = x - q s
+// reaches half a step it decides (it is exact there: x and q s are on grids no
+// finer than s 2^-24). Returns the sum, whose low byte is the code.
+constexpr float kMagic = 12582912.f;
+__device__ __forceinline__ float code_sum(float x, float s, float inv, float &r) {
+  const float t = fmaf(x, inv, kMagic);
+  r = fmaf(kMagic - t, s, x);
+  return t;
+}
+__device__ __noinline__ float code_exact(float x, float s, float inv) {
+  float r;
+  float q = code_sum(x, s, inv, r) - kMagic;
+  const float h = 0.5f * s;
+  const bool odd = (static_cast<int>(q) & 1) != 0;
+  if (r > h || (r == h && odd)) q += 1.f;
+  else if (r < -h || (r == -h && odd)) q -= 1.f;
+  return q + kMagic;
+}
+// four codes, first in the low byte
+__device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s, float inv) {
+  float t[4], r[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) t[k] = code_sum(x[k], s, inv, r[k]);
+  const float far = fmaxf(fmaxf(fabsf(r[0]), fabsf(r[1])), fmaxf(fabsf(r[2]), fabsf(r[3])));
+  if (far >= 0.5f * s) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = code_exact(x[k], s, inv);
   }
-  return static_cast<int>(q);
+  return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
+                     __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+}
+
+// largest |x| of a 16-byte vector, as the bits of the type (monotonic; an
+// infinity or a NaN beats every number)
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const uint4 &w, uint32_t top) {
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t m = 0x7fffffffu;
+    return max(max(max(w.x & m, w.y & m), max(w.z & m, w.w & m)), top);
+  } else {
+    const uint32_t m = 0x7fff7fffu;  // two at a time
+    return __vmaxu2(__vmaxu2(__vmaxu2(w.x & m, w.y & m), __vmaxu2(w.z & m, w.w & m)), top);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t bits_of(T v) {
+  if constexpr (sizeof(T) == 4)
+    return __float_as_uint(v) & 0x7fffffffu;
+  else
+    return *reinterpret_cast<const uint16_t *>(&v) & 0x7fffu;
+}
+template <typename T>
+__device__ __forceinline__ float from_bits(uint32_t b) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(b);
+  } else {
+    const uint16_t h = (uint16_t)b;
+    return to_f32(*reinterpret_cast<const T *>(&h));
+  }
 }
 
 constexpr int kQuantThreads = 256;
-constexpr int kKeep = 4;  // 16-byte vectors of a row that a thread keeps
 
-// One team of TEAM threads per row. VEC: rows start on 16-byte boundaries.
-template <typename T, int TEAM, bool VEC>
+// One team of TEAM threads per row. VEC: rows start on 16-byte boundaries, and
+// a thread keeps KEEP vectors of its row between the two steps.
+template <typename T, int TEAM, bool VEC, int KEEP>
 __global__ void __launch_bounds__(kQuantThreads)
 quant_rows_kernel(const T *__restrict__ x, long long rows, int K, int pitch,
                   int8_t *__restrict__ q, float *__restrict__ scale) {
@@ -80,34 +128,23 @@ quant_rows_kernel(const T *__restrict__ x, long long rows, int K, int pitch,
   const long long row = (long long)blockIdx.x * TEAMS + threadIdx.x / TEAM;
   const bool live = row < rows;
   const T *xr = x + (live ? row : 0) * K;
-  uint32_t top = 0;  // largest |x| as bits: an infinity or NaN beats every number
-  uint4 keep[kKeep];
-  const int nv = VEC ? K / E : 0;
-  if (live) {
-    if (VEC) {
+  const uint4 *xv = reinterpret_cast<const uint4 *>(xr);
+  uint32_t top = 0;
+  uint4 keep[KEEP];
+  const int nv = VEC && live ? K / E : 0;
+  if (VEC) {
 #pragma unroll
-      for (int i = 0; i < kKeep; ++i) {
-        const int v = tid + i * TEAM;
-        keep[i] = v < nv ? __ldg(reinterpret_cast<const uint4 *>(xr) + v) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < kKeep; ++i) {
-        const T *e = reinterpret_cast<const T *>(&keep[i]);
-#pragma unroll
-        for (int k = 0; k < E; ++k)
-          top = max(top, __float_as_uint(to_f32(e[k])) & 0x7fffffffu);
-      }
-      for (int v = tid + kKeep * TEAM; v < nv; v += TEAM) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(xr) + v);
-        const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-        for (int k = 0; k < E; ++k)
-          top = max(top, __float_as_uint(to_f32(e[k])) & 0x7fffffffu);
-      }
-    } else {
-      for (int k = tid; k < K; k += TEAM)
-        top = max(top, __float_as_uint(to_f32(xr[k])) & 0x7fffffffu);
+    for (int i = 0; i < KEEP; ++i) {
+      const int v = tid + i * TEAM;
+      keep[i] = v < nv ? __ldg(xv + v) : make_uint4(0, 0, 0, 0);
     }
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) top = top_of<T>(keep[i], top);
+    for (int v = tid + KEEP * TEAM; v < nv; v += TEAM) top = top_of<T>(__ldg(xv + v), top);
+    if (sizeof(T) == 2) top = max(top & 0xffffu, top >> 16);
+  } else if (live) {
+#pragma unroll 4
+    for (int k = tid; k < K; k += TEAM) top = max(top, bits_of(xr[k]));
   }
   top = __reduce_max_sync(~0u, top);
   if (TEAM > 32) {
@@ -117,44 +154,39 @@ quant_rows_kernel(const T *__restrict__ x, long long rows, int K, int pitch,
     for (int i = 0; i < TEAM / 32; ++i) top = max(top, smax[threadIdx.x / TEAM * (TEAM / 32) + i]);
   }
   if (!live) return;
-  const bool finite = top < 0x7f800000u;
-  const float s = finite ? fmaxf(__uint_as_float(top) / 127.f, 1.17549435e-38f)
-                         : __uint_as_float(0x7fc00000u);
+  const float big = from_bits<T>(top);
+  const bool finite = big < INFINITY;  // false for NaN too
+  const float s = finite ? fmaxf(big / 127.f, 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
   if (tid == 0) scale[row] = s;
   const float inv = 1.f / s;
   int8_t *qr = q + row * pitch;
-  auto code = [&](float v) { return finite ? code_of(v, s, inv) : 0; };
   if (VEC) {
     auto put = [&](int v, const uint4 &w) {
       const T *e = reinterpret_cast<const T *>(&w);
       uint32_t p[E / 4];
 #pragma unroll
-      for (int k = 0; k < E; k += 4)
-        p[k / 4] = (uint32_t)(code(to_f32(e[k])) & 255) |
-                   (uint32_t)(code(to_f32(e[k + 1])) & 255) << 8 |
-                   (uint32_t)(code(to_f32(e[k + 2])) & 255) << 16 |
-                   (uint32_t)(code(to_f32(e[k + 3])) & 255) << 24;
+      for (int k = 0; k < E; k += 4) {
+        const float f[4] = {to_f32(e[k]), to_f32(e[k + 1]), to_f32(e[k + 2]), to_f32(e[k + 3])};
+        p[k / 4] = finite ? codes4(f, s, inv) : 0u;
+      }
       if constexpr (E == 8)
         reinterpret_cast<uint2 *>(qr)[v] = make_uint2(p[0], p[1]);
       else
         reinterpret_cast<uint32_t *>(qr)[v] = p[0];
     };
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
+    for (int i = 0; i < KEEP; ++i) {
       const int v = tid + i * TEAM;
       if (v < nv) put(v, keep[i]);
     }
-    for (int v = tid + kKeep * TEAM; v < nv; v += TEAM)
-      put(v, __ldg(reinterpret_cast<const uint4 *>(xr) + v));
-    // the pad behind K (K is a multiple of 4 or 8 here)
-    for (int k = K + tid; k < pitch; k += TEAM) qr[k] = 0;
+    for (int v = tid + KEEP * TEAM; v < nv; v += TEAM) put(v, __ldg(xv + v));
+    for (int k = K + tid; k < pitch; k += TEAM) qr[k] = 0;  // the pad behind K
   } else {
     for (int k = 4 * tid; k < pitch; k += 4 * TEAM) {
-      uint32_t p = 0;
+      float f[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (k + j < K) p |= (uint32_t)(code(to_f32(xr[k + j])) & 255) << (8 * j);
-      *reinterpret_cast<uint32_t *>(qr + k) = p;
+      for (int j = 0; j < 4; ++j) f[j] = k + j < K ? to_f32(xr[k + j]) : 0.f;
+      *reinterpret_cast<uint32_t *>(qr + k) = finite ? codes4(f, s, inv) : 0u;
     }
   }
 }
@@ -163,21 +195,22 @@ template <typename T>
 int launch_quant(const void *x, long long rows, int K, int8_t *q, float *scale, cudaStream_t st) {
   const int pitch = (K + 15) / 16 * 16;
   const T *xt = static_cast<const T *>(x);
-  const bool vec = aligned(x, 16) && (size_t)K * sizeof(T) % 16 == 0;
-  // a warp per row while its lanes can keep the row; else a CTA per row
-  const bool warp = (size_t)K * sizeof(T) <= 32 * 16 * kKeep;
-  const long long blocks = warp ? (rows + 7) / 8 : rows;
-  if (warp) {
-    if (vec)
-      quant_rows_kernel<T, 32, true><<<blocks, kQuantThreads, 0, st>>>(xt, rows, K, pitch, q, scale);
-    else
-      quant_rows_kernel<T, 32, false><<<blocks, kQuantThreads, 0, st>>>(xt, rows, K, pitch, q, scale);
-  } else {
-    if (vec)
-      quant_rows_kernel<T, 256, true><<<blocks, kQuantThreads, 0, st>>>(xt, rows, K, pitch, q, scale);
-    else
-      quant_rows_kernel<T, 256, false><<<blocks, kQuantThreads, 0, st>>>(xt, rows, K, pitch, q, scale);
-  }
+  const size_t bytes = (size_t)K * sizeof(T);
+  const bool vec = aligned(x, 16) && bytes % 16 == 0;
+  // a warp per row while its lanes can keep the row (16 vectors each: 8 KB),
+  // else a CTA per row
+  const unsigned warps = (unsigned)((rows + 7) / 8), ctas = (unsigned)rows;
+  constexpr int B = kQuantThreads;
+  if (vec && bytes <= 32 * 16 * 4)
+    quant_rows_kernel<T, 32, true, 4><<<warps, B, 0, st>>>(xt, rows, K, pitch, q, scale);
+  else if (vec && bytes <= 32 * 16 * 16 && rows >= 8 * sm_count())
+    quant_rows_kernel<T, 32, true, 16><<<warps, B, 0, st>>>(xt, rows, K, pitch, q, scale);
+  else if (vec)
+    quant_rows_kernel<T, 256, true, 8><<<ctas, B, 0, st>>>(xt, rows, K, pitch, q, scale);
+  else if (bytes <= 32 * 16 * 4)
+    quant_rows_kernel<T, 32, false, 1><<<warps, B, 0, st>>>(xt, rows, K, pitch, q, scale);
+  else
+    quant_rows_kernel<T, 256, false, 1><<<ctas, B, 0, st>>>(xt, rows, K, pitch, q, scale);
   return check_launch("quant_rows_kernel");
 }
 
@@ -192,7 +225,7 @@ int quant_rows(const void *x, int dtype, long long rows, int K, int8_t *q, float
 constexpr int kBM = 128;
 constexpr int kEpiWarp0 = 2, kEpiWarps = 8;
 constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
-constexpr int kPitchW = 33;  // words of a staged row piece (32 and one against bank conflicts)
+constexpr int kPitchW = 36;  // words of a staged row piece: 32, and 4 against bank conflicts
 
 template <int BN>
 struct Cfg {
@@ -215,39 +248,50 @@ struct LinParams {
   int N, ksteps, K;
   long long tiles_n, tiles;
   int act;
+  bool vec;          // rows of y start on 16-byte boundaries
   int *err;
 };
 
-// One 32-row piece of y of 32 words per row, staged by the calling warp at
-// stg (row pitch kPitchW words), to global memory; the piece's columns
-// [col, col + PC) of the row, clipped at N.
+// One 32-row piece of y (32 words per row at most, PC columns from `col` on,
+// clipped at N), staged by the calling warp at stg (row pitch kPitchW words),
+// to global memory. vec: every row of y starts on a 16-byte boundary.
 template <typename T, int PC>
 __device__ __forceinline__ void write_piece(T *y, long long row0, long long rows, int N, int col,
-                                            const uint32_t *stg, int lane) {
-  const int n = min(N - col, PC);  // elements of a row of the piece
+                                            bool vec, const uint32_t *stg, int lane) {
+  constexpr int PER = 4 / sizeof(T);      // elements per word
+  constexpr int W = PC / PER;             // words of a row
+  const int n = min(N - col, PC);         // elements of a row
   const int nr = (int)min((long long)32, rows - row0);
   T *o = y + row0 * N + col;
-  if constexpr (sizeof(T) == 4) {
+  if (vec && n == PC) {
+    constexpr int LPR = W / 4, RPI = 32 / LPR;  // lanes per row, rows per instruction
+    const int r = lane / LPR, w = lane % LPR * 4;
+#pragma unroll 8
+    for (int r0 = 0; r0 < 32; r0 += RPI)
+      if (r0 + r < nr)
+        *reinterpret_cast<uint4 *>(reinterpret_cast<uint32_t *>(o + (long long)(r0 + r) * N) + w) =
+            *reinterpret_cast<const uint4 *>(stg + (r0 + r) * kPitchW + w);
+  } else if constexpr (PER == 1) {
     if (lane < n)
-      for (int r = 0; r < nr; ++r, o += N)
-        reinterpret_cast<uint32_t *>(o)[lane] = stg[r * kPitchW + lane];
+#pragma unroll 8
+      for (int r = 0; r < 32; ++r)
+        if (r < nr) reinterpret_cast<uint32_t *>(o + (long long)r * N)[lane] = stg[r * kPitchW + lane];
   } else {
-  for (int r = 0; r < nr; ++r, o += N) {
-    const uint32_t *s = stg + r * kPitchW;
-    if ((reinterpret_cast<uintptr_t>(o) & 3) == 0) {
-      if (2 * lane + 1 < n)
-        reinterpret_cast<uint32_t *>(o)[lane] = s[lane];
-      else if (2 * lane < n)
-        reinterpret_cast<uint16_t *>(o)[2 * lane] = (uint16_t)s[lane];
-    } else {  // words one element further on
-      if (2 * lane + 2 < n)
-        *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(o) + 2 * lane + 1) =
-            __byte_perm(s[lane], s[lane + 1], 0x5432);
-      else if (2 * lane + 1 < n)
-        reinterpret_cast<uint16_t *>(o)[2 * lane + 1] = (uint16_t)(s[lane] >> 16);
-      if (lane == 0) reinterpret_cast<uint16_t *>(o)[0] = (uint16_t)s[0];
+    // 4-byte stores on 4-byte boundaries: a row that starts between two takes
+    // its words one element further on, and its first element on its own
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      if (r >= nr) break;
+      uint16_t *orow = reinterpret_cast<uint16_t *>(o + (long long)r * N);
+      const uint32_t a = stg[r * kPitchW + lane], b = stg[r * kPitchW + lane + 1];
+      const int odd = (int)(reinterpret_cast<uintptr_t>(orow) >> 1) & 1;
+      const int e = 2 * lane + odd;
+      if (e + 1 < n)
+        *reinterpret_cast<uint32_t *>(orow + e) = odd ? __byte_perm(a, b, 0x5432) : a;
+      else if (e < n)
+        orow[e] = (uint16_t)(odd ? a >> 16 : a);
+      if (odd && lane == 0) orow[0] = (uint16_t)a;
     }
-  }
   }
 }
 
@@ -271,8 +315,6 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-template <>
-__device__ __forceinline__ uint32_t pack2<float>(float lo, float) { return __float_as_uint(lo); }
 
 // SMALLK: |sum| < 2^22, so an s32 becomes fp32 by adding it to the bits of
 // 1.5 * 2^23 (two full-rate instructions; the conversion instruction runs at an
@@ -316,7 +358,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
   const int KS = p.ksteps;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       tma_prefetch_desc(&xmap);
       tma_prefetch_desc(&wmap);
       long long j = 0;
@@ -344,7 +386,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = idesc_i8(kBM, BN);
       long long j = 0;
       int i = 0;
@@ -406,6 +448,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
           uint32_t v[32];
           tmem_ld32(ta + c + g, v);
           tmem_ld_wait(v);
+          uint32_t o[32 / PER];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float4 cc = *reinterpret_cast<const float4 *>(&cols[g + e]);
@@ -415,16 +458,20 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
                                     : (float)(int)v[e + 1];
             const float y0 = activate(fmaf(a0 * sx, cc.x, cc.y), p.act);
             const float y1 = activate(fmaf(a1 * sx, cc.z, cc.w), p.act);
-            if (PER == 2) {
-              stg[lane * kPitchW + (g + e) / 2] = pack2<T>(y0, y1);
+            if constexpr (PER == 2) {
+              o[e / 2] = pack2<T>(y0, y1);
             } else {
-              stg[lane * kPitchW + e] = __float_as_uint(y0);
-              stg[lane * kPitchW + e + 1] = __float_as_uint(y1);
+              o[e] = __float_as_uint(y0);
+              o[e + 1] = __float_as_uint(y1);
             }
           }
+          uint4 *so = reinterpret_cast<uint4 *>(stg + lane * kPitchW + g / PER);
+#pragma unroll
+          for (int e = 0; e < 8 / PER; ++e)
+            so[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
         __syncwarp();
-        if (row0 < p.rows) write_piece<T, PC>(y, row0, p.rows, p.N, n0 + c, stg, lane);
+        if (row0 < p.rows) write_piece<T, PC>(y, row0, p.rows, p.N, n0 + c, p.vec, stg, lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -513,6 +560,7 @@ int run_product(const void *xq, const float *sx, long long rows, int K, const vo
   p.K = K;
   p.ksteps = (K + 127) / 128;
   p.act = act;
+  p.vec = aligned(y, 16) && (size_t)N * (out_dtype == TOCR_DTYPE_F32 ? 4 : 2) % 16 == 0;
   p.err = err;
   const int pitch = (K + 15) / 16 * 16;
   if (out_dtype == TOCR_DTYPE_F16) return product<__half>(xq, wq, p, pitch, st);

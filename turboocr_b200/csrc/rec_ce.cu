@@ -55,11 +55,14 @@ using namespace ptx;
 
 constexpr int kTile = 128;       // rows of a stationary tile (MMA M, TMEM lanes)
 constexpr int kEpiWarp0 = 2;
-constexpr int kEpiWarps = 16;    // two groups of eight; a group takes every other chunk
+constexpr int kEpiWarps = 16;    // forward: two groups of eight that take every other chunk
 constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
 constexpr int kEpiThreads = 32 * kEpiWarps;
 constexpr int kTmemCols = 512;
+constexpr int kPolyPairs = 2;    // of 16 pairs of exponentials, those not left to the special-function unit
+constexpr int kColSlots = 8;     // ring of the streamed rows' per-row terms
 constexpr int kRowBlock = 256;   // rows per block of the numbering kernels
+constexpr int kDirect = 4;       // blocks whose rows the placing kernel counts itself
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxK = 256;
@@ -81,9 +84,9 @@ struct Workspace {
   float *gblk;
   int *rowidx;     // [rows_pad] the row of each kept row
   int *tgt;        // [rows_pad] its target (-1 behind the last)
+  float *bias2;    // [V to 128] bias * log2(e), -inf behind the last class
   // forward
-  float *lt;       // [rows_pad] target logit * log2(e)
-  float2 *part;    // [tiles + grid][128] (max, sum) of a range's piece of a tile
+  float2 *part;    // [tiles + grid][128] (base, sum) of a range's piece of a tile
   // backward
   uint8_t *xc;     // [rows_pad][K] the kept rows of F, zero behind the last
   float *nlse;     // [rows_pad] -lse * log2(e) (-inf behind the last)
@@ -95,7 +98,7 @@ struct Workspace {
 };
 
 // Layout of the caller's workspace for `rows` rows; base may be null (sizes).
-inline Workspace carve(uint8_t *base, long long rows, int K, bool backward) {
+inline Workspace carve(uint8_t *base, long long rows, int K, int V, bool backward) {
   constexpr int grid = kMaxGrid;
   Workspace w{};
   size_t off = 0;
@@ -112,8 +115,8 @@ inline Workspace carve(uint8_t *base, long long rows, int K, bool backward) {
   w.gblk = reinterpret_cast<float *>(take(blocks * 4));
   w.rowidx = reinterpret_cast<int *>(take(pad * 4));
   w.tgt = reinterpret_cast<int *>(take(pad * 4));
+  w.bias2 = reinterpret_cast<float *>(take(((size_t)V + 127) / 128 * 128 * 4));
   if (!backward) {
-    w.lt = reinterpret_cast<float *>(take(pad * 4));
     w.part = reinterpret_cast<float2 *>(take((size_t)(pad / kTile + grid) * kTile * 8));
   } else {
     w.xc = take((size_t)pad * K * 2);
@@ -137,7 +140,9 @@ __device__ __forceinline__ int target_of(const void *t, bool wide, long long i, 
   return v >= 0 && v < V ? v : -1;
 }
 
-// Kept rows and largest weight of every block of 256 rows.
+// Kept rows and largest weight of every block of 256 rows (calls of more than
+// kDirect blocks; below that the placing kernel counts for itself, which saves
+// a launch).
 __global__ void __launch_bounds__(kRowBlock)
 ce_count_kernel(const void *targets, bool wide, int rows, int V, const float *g, int *cnt,
                 float *gblk) {
@@ -162,10 +167,13 @@ struct PlaceParams {
   bool wide;
   int rows, V, K;
   float shift;       // 2^14 for fp16, 1 for bf16
+  bool direct;       // no cnt, gblk: count here
   const int *cnt;
   const float *gblk;
   Header *hdr;
   int *rowidx, *tgt;
+  const float *bias;
+  float *bias2;
   // forward: outputs of the padding rows
   float *loss, *lse_out;
   // backward
@@ -177,6 +185,8 @@ struct PlaceParams {
 
 // Numbers the kept rows in their order and writes what the products take of
 // each (backward: a copy of its features); padding rows get their zero outputs.
+// The bias goes to the log2 domain, padded to whole chunks.
+// blockIdx.x: 256 rows; y: a share of the copying (share 0 writes the rest).
 template <bool BWD>
 __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p) {
   __shared__ int swarp[kRowBlock / 32];
@@ -187,9 +197,19 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
   // kept rows before this block, and the largest weight of all
   int before = 0;
   float gm = 0.f;
-  for (int b = tid; b < (int)gridDim.x; b += kRowBlock) {
-    if (b < (int)blockIdx.x) before += p.cnt[b];
-    if (BWD) gm = fmaxf(gm, p.gblk[b]);
+  if (p.direct) {
+    const int mine = blockIdx.x * kRowBlock, upto = BWD ? p.rows : mine;
+#pragma unroll 4
+    for (int k = tid; k < upto; k += kRowBlock) {
+      if (target_of(p.targets, p.wide, k, p.V) < 0) continue;
+      if (k < mine) ++before;
+      if (BWD) gm = fmaxf(gm, fabsf(p.g[k]));
+    }
+  } else {
+    for (int b = tid; b < (int)gridDim.x; b += kRowBlock) {
+      if (b < (int)blockIdx.x) before += p.cnt[b];
+      if (BWD) gm = fmaxf(gm, p.gblk[b]);
+    }
   }
   if (tid == 0) s_off = 0;
   __syncthreads();
@@ -222,7 +242,11 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
   __syncthreads();
   const int off = s_off;
   const int dst = t >= 0 ? off + rank : -1;
-  if (i < p.rows) {
+  const bool share0 = blockIdx.y == 0;
+  for (int v = (blockIdx.y * gridDim.x + blockIdx.x) * kRowBlock + tid; v < (p.V + 127) / 128 * 128;
+       v += gridDim.x * gridDim.y * kRowBlock)
+    p.bias2[v] = v < p.V ? (p.bias ? p.bias[v] * kLog2e : 0.f) : -INFINITY;
+  if (share0 && i < p.rows) {
     if (t >= 0) {
       p.rowidx[dst] = (int)i;
       p.tgt[dst] = t;
@@ -239,13 +263,13 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
   }
   const bool last = blockIdx.x == gridDim.x - 1;
   const int n = off + s_total;  // all kept rows, in the last block
-  if (last && tid == 0) {
+  if (last && share0 && tid == 0) {
     p.hdr->n = n;
     p.hdr->gmax = s_gmax;
   }
   // the unused rows up to the end of the last tile
   const int end = max(kTile, (n + kTile - 1) / kTile * kTile);
-  if (last) {
+  if (last && share0) {
     for (int j = n + tid; j < end; j += kRowBlock) {
       p.rowidx[j] = -1;
       p.tgt[j] = -1;
@@ -262,7 +286,8 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
     const int q = p.K / 8;  // 16-byte pieces of a row
     const int here = (int)min((long long)kRowBlock, (long long)p.rows - row0);
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int e = tid; e < here * q; e += kRowBlock) {
+    const int from = blockIdx.y * kRowBlock + tid, step = gridDim.y * kRowBlock;
+    for (int e = from; e < here * q; e += step) {
       const int r = e / q, c = e - r * q;
       const int d = s_dst[r];
       if (d >= 0)
@@ -272,22 +297,32 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
         reinterpret_cast<uint4 *>(p.dfeat)[(size_t)(row0 + r) * q + c] = zero;
     }
     if (last)
-      for (long long e = tid; e < (long long)(end - n) * q; e += kRowBlock)
+      for (int e = from; e < (end - n) * q; e += step)
         reinterpret_cast<uint4 *>(p.xc)[(size_t)n * q + e] = zero;
   }
 }
 
 // ------------------------------------------------------------ step line -----
-// Steps [begin, end) of the line of CTA c out of G.
-__host__ __device__ __forceinline__ long long cut(long long total, int c, int G) {
-  return total / G * c + total % G * c / G;
-}
-// The CTA whose range holds step `it`.
-__device__ __forceinline__ int owner(long long total, long long it, int G) {
-  int c = (int)(it / (total / G + 1));
-  while (c + 1 < G && cut(total, c + 1, G) <= it) ++c;
-  return c;
-}
+// The line of `total` steps in G ranges of equal length (to one step). G is
+// the grid, or the steps where they are fewer, so that no range is empty.
+struct Cuts {
+  long long total, q, r;
+  int G;
+  __device__ Cuts(long long steps, int grid) {
+    total = steps;
+    G = (int)min((long long)grid, steps);
+    q = G ? total / G : 0;
+    r = G ? total - q * G : 0;
+  }
+  // first step of range c
+  __device__ long long at(int c) const { return c >= G ? total : q * c + r * c / G; }
+  // the range that holds step `it`
+  __device__ int owner(long long it) const {
+    int c = (int)(it / (q + 1));
+    while (c + 1 < G && at(c + 1) <= it) ++c;
+    return c;
+  }
+};
 
 // ------------------------------------------------------------ small parts ---
 __device__ __forceinline__ float ex2(float x) {
@@ -329,6 +364,65 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return r;
 }
 
+// y = l * log2(e) + terms of 32 columns, in pairs
+__device__ __forceinline__ void logits32(uint64_t (&y)[16], const uint32_t (&v)[32],
+                                         const float *terms) {
+  const uint64_t l2e2 = pk(kLog2e, kLog2e);
+  const ulonglong2 *cq = reinterpret_cast<const ulonglong2 *>(terms);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const ulonglong2 c = cq[q];
+    y[2 * q] = fma2(pk(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1])), l2e2, c.x);
+    y[2 * q + 1] =
+        fma2(pk(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])), l2e2, c.y);
+  }
+}
+// exp2 of a pair without the special-function unit: y = n + f, |f| <= 1/2, by
+// adding and taking off 1.5 * 2^23; exp2(f) by its Taylor polynomial in f ln 2
+// up to f^6 (the next term is 1.2e-7 at |f| = 1/2, half a step of the result);
+// n goes into the exponent. y below -126 counts as -126 (2^-126 instead of
+// less), y up to 127.
+__device__ __forceinline__ uint64_t ex2_poly(uint64_t y) {
+  float a, b;
+  upk(y, a, b);
+  y = pk(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t t = add2(y, pk(12582912.f, 12582912.f));
+  const uint64_t n = add2(t, pk(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pk(-1.f, -1.f), y);
+  uint64_t r = pk(1.5403530e-4f, 1.5403530e-4f);
+  r = fma2(r, f, pk(1.3333558e-3f, 1.3333558e-3f));
+  r = fma2(r, f, pk(9.6181291e-3f, 9.6181291e-3f));
+  r = fma2(r, f, pk(5.5504109e-2f, 5.5504109e-2f));
+  r = fma2(r, f, pk(2.4022651e-1f, 2.4022651e-1f));
+  r = fma2(r, f, pk(6.9314718e-1f, 6.9314718e-1f));
+  r = fma2(r, f, pk(1.f, 1.f));
+  float r0, r1, t0, t1;
+  upk(r, r0, r1);
+  upk(t, t0, t1);
+  return pk(__uint_as_float(__float_as_uint(r0) + (__float_as_uint(t0) << 23)),
+            __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23)));
+}
+// adds exp2(y) (exp2(y - base), nb = -base twice) of 32 columns to four sums
+template <bool BASE>
+__device__ __forceinline__ void add_exp(uint64_t (&s)[4], const uint64_t (&y)[16], uint64_t nb) {
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const uint64_t z = BASE ? add2(y[q], nb) : y[q];
+    if (q % 16 < kPolyPairs) {
+      s[q & 3] = add2(s[q & 3], ex2_poly(z));
+    } else {
+      float a, b;
+      upk(z, a, b);
+      s[q & 3] = add2(s[q & 3], pk(ex2(a), ex2(b)));
+    }
+  }
+}
+__device__ __forceinline__ float sum4(const uint64_t (&s)[4]) {
+  float a, b;
+  upk(add2(add2(s[0], s[1]), add2(s[2], s[3])), a, b);
+  return a + b;
+}
+
 // One warp's share of a stationary tile into tensor memory: lane = row, the
 // warp's quarter `w4` of the features (8 * KA columns of two features).
 // src: this lane's row, or null for a zero row.
@@ -347,14 +441,17 @@ __device__ __forceinline__ void load_tile_tmem(uint32_t tx, const uint8_t *src, 
   }
 }
 
-// Waits (bounded) until the loads that the producer issued and nobody waited
-// for have landed: a CTA that gives up leaves no copy in flight into its
-// shared memory.
-__device__ __forceinline__ void drain_loads(uint64_t *b_full, long long issued, int stages) {
-  const long long first = issued > stages ? issued - stages : 0;
-  for (long long n = first; n < issued; ++n) {
+// Waits (bounded) until every load that was issued into a ring has landed, `at`
+// being the slot after the last one: a CTA that gives up leaves no copy in
+// flight into its shared memory.
+template <int N>
+__device__ __forceinline__ void drain_loads(uint64_t *full, const Ring<N> &at) {
+  for (int s = 0; s < N; ++s) {
+    const bool wrapped = s >= at.i;  // last filled one round ago, if at all
+    if (wrapped && at.first) continue;
+    const uint32_t parity = wrapped ? at.phase ^ 1 : at.phase;
     const long long t0 = clock64();
-    while (!mbar_try_wait(&b_full[n % stages], (uint32_t)(n / stages) & 1))
+    while (!mbar_try_wait(&full[s], parity))
       if (clock64() - t0 > (1ll << 30)) break;
   }
 }
@@ -368,20 +465,20 @@ struct FwdCfg {
   static constexpr int STAGES = KA == 1 ? 8 : KA == 2 ? 6 : KA == 3 ? 4 : 3;
   static constexpr int NBUF = 3;                      // S buffers
   static constexpr int TX = 0, TS = 128;              // TMEM columns: features, S buffers
-  static constexpr int OFF_BAR = STAGES * STAGE;
-  static constexpr int NBAR = 2 * STAGES + 2 * NBUF + 1;
+  static constexpr int OFF_COL = STAGES * STAGE;                    // [kColSlots][CN] floats
+  static constexpr int OFF_COMB = OFF_COL + kColSlots * CN * 4;     // [2][4][2][128] floats
+  static constexpr int OFF_BAR = OFF_COMB + 2 * 4 * 2 * kTile * 4;
+  static constexpr int NBAR = 2 * STAGES + 2 * NBUF + 2 * kColSlots + 1;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-  static constexpr int OFF_COMB = (OFF_MISC + 16 + 15) / 16 * 16;   // [2][4][2][128] floats
-  static constexpr int OFF_COL = OFF_COMB + 2 * 4 * 2 * kTile * 4;  // [16][32] floats
-  static constexpr int SMEM = OFF_COL + kEpiWarps * 32 * 4 + 1024;
+  static constexpr int SMEM = OFF_MISC + 16 + 1024;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 struct FwdParams {
   const uint8_t *feat;
-  const float *bias;
+  const float *bias2;
   const Header *hdr;
-  const int *rowidx, *tgt;
-  float *lt;
+  const int *rowidx;
   float2 *part;
   int V, K, chunks;
   int *err;
@@ -398,11 +495,13 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
   uint64_t *b_empty = b_full + C::STAGES;
   uint64_t *s_full = b_empty + C::STAGES;
   uint64_t *s_empty = s_full + C::NBUF;
-  uint64_t *x_ready = s_empty + C::NBUF;
+  uint64_t *c_full = s_empty + C::NBUF;
+  uint64_t *c_empty = c_full + kColSlots;
+  uint64_t *x_ready = c_empty + kColSlots;
   uint32_t *s_tmem = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
   volatile int *s_abort = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 4);
   float *comb = reinterpret_cast<float *>(smem + C::OFF_COMB);
-  float *scol = reinterpret_cast<float *>(smem + C::OFF_COL);
+  const float *scol = reinterpret_cast<const float *>(smem + C::OFF_COL);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -413,6 +512,10 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
     for (int b = 0; b < C::NBUF; ++b) {
       mbar_init(&s_full[b], 1);
       mbar_init(&s_empty[b], kEpiWarps / 2);
+    }
+    for (int b = 0; b < kColSlots; ++b) {
+      mbar_init(&c_full[b], 1);
+      mbar_init(&c_empty[b], kEpiWarps / 2);
     }
     mbar_init(x_ready, kEpiWarps);
     *s_abort = 0;
@@ -429,49 +532,64 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
   const int n = p.hdr->n;
   const int NC = p.chunks;
   const long long total = (long long)((n + kTile - 1) / kTile) * NC;
-  const long long it0 = cut(total, blockIdx.x, gridDim.x);
-  const long long it1 = cut(total, blockIdx.x + 1, gridDim.x);
+  const Cuts cuts(total, gridDim.x);
+  const long long it0 = cuts.at(blockIdx.x), it1 = cuts.at(blockIdx.x + 1);
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       tma_prefetch_desc(&wmap);
-      long long j = 0;
-      for (long long it = it0; it < it1; ++it, ++j) {
-        const int s = (int)(j % C::STAGES);
-        const uint32_t u = (uint32_t)(j / C::STAGES);
-        if (u > 0 && !mbar_wait_bounded(&b_empty[s], (u - 1) & 1, s_abort, p.err, 61)) break;
-        mbar_arrive_expect_tx(&b_full[s], C::STAGE);
-        const int c = (int)(it % NC);
+      Ring<C::STAGES> bs;
+      Ring<kColSlots> cr;
+      int c = (int)(it0 % NC);
+      for (int left = (int)(it1 - it0); left > 0; --left) {
+        if (!bs.first && !mbar_wait_bounded(&b_empty[bs.i], bs.phase ^ 1, s_abort, p.err, 61)) break;
+        mbar_arrive_expect_tx(&b_full[bs.i], C::STAGE);
+        uint8_t *dst = smem + bs.i * C::STAGE;
+#pragma unroll
         for (int k = 0; k < KA; ++k)
-          tma_load_2d(smem + s * C::STAGE + k * C::CN * 128, &wmap, &b_full[s], 64 * k, c * C::CN);
+          tma_load_2d(dst + k * C::CN * 128, &wmap, &b_full[bs.i], 64 * k, c * C::CN);
+        bs.next();
+        if (!cr.first && !mbar_wait_bounded(&c_empty[cr.i], cr.phase ^ 1, s_abort, p.err, 66)) break;
+        mbar_arrive_expect_tx(&c_full[cr.i], C::CN * 4);
+        bulk_load(smem + C::OFF_COL + cr.i * C::CN * 4, p.bias2 + (size_t)c * C::CN, C::CN * 4,
+                  &c_full[cr.i]);
+        cr.next();
+        if (++c == NC) c = 0;
       }
-      if (*s_abort) drain_loads(b_full, j, C::STAGES);
+      if (*s_abort) {
+        drain_loads(b_full, bs);
+        drain_loads(c_full, cr);
+      }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = BF16 ? idesc_bf16(kTile, C::CN) : idesc_f16(kTile, C::CN);
-      long long j = 0;
+      Ring<C::STAGES> bs;
+      Ring<C::NBUF> sr;
+      const uint64_t bdesc = sw128_kmajor_desc(smem_u32(smem));
       uint32_t seg = 0;
-      bool ok = true;
-      for (long long it = it0; ok && it < it1; ++it, ++j) {
-        if (it == it0 || it % NC == 0) {
-          ok = mbar_wait_bounded(x_ready, seg & 1, s_abort, p.err, 62);
+      int left_tile = NC - (int)(it0 % NC);  // chunks left of the tile
+      bool fresh = true;
+      for (int left = (int)(it1 - it0); left > 0; --left) {
+        if (fresh) {
+          if (!mbar_wait_bounded(x_ready, seg & 1, s_abort, p.err, 62)) break;
           ++seg;
-          if (!ok) break;
         }
-        const int s = (int)(j % C::STAGES), b = (int)(j % C::NBUF);
-        const uint32_t u = (uint32_t)(j / C::STAGES), ub = (uint32_t)(j / C::NBUF);
-        if (!mbar_wait_bounded(&b_full[s], u & 1, s_abort, p.err, 63)) break;
-        if (ub > 0 && !mbar_wait_bounded(&s_empty[b], (ub - 1) & 1, s_abort, p.err, 64)) break;
+        if (!mbar_wait_bounded(&b_full[bs.i], bs.phase, s_abort, p.err, 63)) break;
+        if (!sr.first && !mbar_wait_bounded(&s_empty[sr.i], sr.phase ^ 1, s_abort, p.err, 64)) break;
         tc_fence_after();
-        const uint32_t baddr = smem_u32(smem + s * C::STAGE);
+        const uint64_t bd = bdesc + (uint64_t)(bs.i * (C::STAGE >> 4));
+        const uint32_t d = tmem + C::TS + sr.i * C::CN;
 #pragma unroll
         for (int k = 0; k < 4 * KA; ++k)
-          mma_f16_ts(tmem + C::TS + b * C::CN, tmem + C::TX + 8 * k,
-                     sw128_kmajor_desc(baddr + (k >> 2) * (C::CN * 128) + 32u * (k & 3)), idesc,
-                     k > 0 ? 1u : 0u);
-        mma_commit(&b_empty[s]);
-        mma_commit(&s_full[b]);
+          mma_f16_ts(d, tmem + C::TX + 8 * k, bd + (((k >> 2) * (C::CN * 128) + 32 * (k & 3)) >> 4),
+                     idesc, k > 0 ? 1u : 0u);
+        mma_commit(&b_empty[bs.i]);
+        mma_commit(&s_full[sr.i]);
+        bs.next();
+        sr.next();
+        fresh = --left_tile == 0;
+        if (fresh) left_tile = NC;
       }
     }
   } else {
@@ -481,122 +599,116 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
     const int quad = warp & 3;           // the TMEM lanes a warp may read
     const int r = quad * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16);
-    float *col = scol + ew * 32;
-    const uint64_t l2e2 = pk(kLog2e, kLog2e);
-    long long j = 0;
-    int seg = 0;
+    Ring<C::NBUF> sr;
+    Ring<kColSlots> cr;
+    int seg = 0, odd = 0;  // odd: parity of the chunk
     bool ok = true;
     for (long long it = it0; it < it1; ++seg) {
       const int tile = (int)(it / NC), c0 = (int)(it % NC);
       const int cnt = (int)min((long long)(NC - c0), it1 - it);
       const int row = tile * kTile + r;  // kept rows are numbered from 0
       const int src = row < n ? p.rowidx[row] : -1;
-      const int tg = row < n ? p.tgt[row] : -1;
       load_tile_tmem<KA>(tl + C::TX, src >= 0 ? p.feat + (size_t)src * p.K * 2 : nullptr, p.K,
                          ew >> 2);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(x_ready);
-      // running maximum of y = l * log2(e), and the sum of exp2(y - base)
-      float my = -INFINITY, sum = 0.f, base = 0.f;
-      for (int i = 0; i < cnt; ++i, ++j) {
-        if ((int)(j & 1) != grp) continue;
-        const int b = (int)(j % C::NBUF);
-        const uint32_t ub = (uint32_t)(j / C::NBUF);
-        const int v0 = (c0 + i) * C::CN + half * 64;
-        float bl[2];
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int v = v0 + 32 * g + lane;
-          bl[g] = v < p.V ? (p.bias ? __ldg(p.bias + v) * kLog2e : 0.f) : -INFINITY;
-        }
-        ok = ok && mbar_wait_bounded(&s_full[b], ub & 1, s_abort, p.err, 65);
+      // sum of exp2(y - base), y = l * log2(e). The base is 0 if the first
+      // logits that the thread sees have their maximum within 2^64 of it, else
+      // that maximum: the sum cannot vanish. It grows with 64 logits whose sum
+      // passes 2^100, so it cannot overflow either, and no maximum is taken of
+      // the others.
+      float sum = 0.f, base = 0.f;
+      bool seen = false;               // this lane has its base
+      bool fresh = true, based = false;  // some lane of the warp has none; one other than 0
+      for (int i = 0; i < cnt; ++i, odd ^= 1, sr.next(), cr.next()) {
+        if (odd != grp) continue;
+        const int b = sr.i, cs = cr.i;
+        ok = ok && mbar_wait_bounded(&s_full[b], sr.phase, s_abort, p.err, 65) &&
+             mbar_wait_bounded(&c_full[cs], cr.phase, s_abort, p.err, 67);
         if (!ok) break;
         tc_fence_after();
         const uint32_t ts = tl + C::TS + b * C::CN + half * 64;
-        uint32_t va[32], vb[32];
-        tmem_ld32(ts, va);
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint32_t(&v)[32] = g ? vb : va;
-          const int cb = v0 + 32 * g;
-          __syncwarp();
-          col[lane] = bl[g];
-          __syncwarp();
+        const float *terms = scol + cs * C::CN + half * 64;
+        float add = 0.f;
+        bool slow = fresh;
+        if (!slow) {
+          const uint64_t nb = pk(-base, -base);
+          uint64_t s4[4] = {0, 0, 0, 0}, y[16];
+          uint32_t v[32], w[32];
+          tmem_ld32(ts, v);
           tmem_ld_wait(v);
-          if (g == 0) tmem_ld32(ts + 32, vb);
-          if (g == 1) {  // all of this warp's columns are in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[b]);
-          }
-          if (cb >= p.V) continue;
-          uint64_t y[16];
-          const ulonglong2 *cq = reinterpret_cast<const ulonglong2 *>(col);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const ulonglong2 bb = cq[q];
-            y[2 * q] = fma2(pk(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1])), l2e2,
-                            bb.x);
-            y[2 * q + 1] = fma2(pk(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])),
-                                l2e2, bb.y);
-          }
-          float f[32];
-#pragma unroll
-          for (int q = 0; q < 16; ++q) upk(y[q], f[2 * q], f[2 * q + 1]);
-          const bool hit = tg >= cb && tg < cb + 32;
-          if (__any_sync(~0u, hit)) {
-            float l = 0.f;
-#pragma unroll
-            for (int q = 0; q < 32; ++q)
-              if (tg == cb + q) l = f[q];
-            if (hit) p.lt[row] = l;
-          }
-          float m[11];
-#pragma unroll
-          for (int q = 0; q < 10; ++q) m[q] = fmaxf(fmaxf(f[3 * q], f[3 * q + 1]), f[3 * q + 2]);
-          m[10] = fmaxf(f[30], f[31]);
-          const float m0 = fmaxf(fmaxf(m[0], m[1]), m[2]), m1 = fmaxf(fmaxf(m[3], m[4]), m[5]);
-          const float m2 = fmaxf(fmaxf(m[6], m[7]), m[8]), m3 = fmaxf(m[9], m[10]);
-          const float gm = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-          if (gm > my) {
-            my = gm;
-            // base stays 0 while the maximum is within 2^64 of it
-            if (my > base + 64.f || my < base - 64.f) {
-              sum = sum > 0.f ? sum * ex2(base - my) : 0.f;
-              base = my;
-            }
-          }
-          uint64_t s4[4] = {0, 0, 0, 0};
-          if (__any_sync(~0u, base != 0.f)) {
-            const uint64_t nb = pk(-base, -base);
+          tmem_ld32(ts + 32, w);
+          logits32(y, v, terms);
+          if (based)
+            add_exp<true>(s4, y, nb);
+          else
+            add_exp<false>(s4, y, nb);
+          tmem_ld_wait(w);
+          logits32(y, w, terms + 32);
+          if (based)
+            add_exp<true>(s4, y, nb);
+          else
+            add_exp<false>(s4, y, nb);
+          add = sum4(s4);
+          slow = __any_sync(~0u, !(add < 0x1p100f));
+        }
+        if (slow) {  // a first or a larger base
+          float gm = -INFINITY;
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g) {
+            uint32_t v[32];
+            uint64_t y[16];
+            tmem_ld32(ts + 32 * g, v);
+            tmem_ld_wait(v);
+            logits32(y, v, terms + 32 * g);
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
-              float a0, a1;
-              upk(add2(y[q], nb), a0, a1);
-              s4[q & 3] = add2(s4[q & 3], pk(ex2(a0), ex2(a1)));
+              float f0, f1;
+              upk(y[q], f0, f1);
+              gm = fmaxf(fmaxf(gm, f0), f1);
             }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 16; ++q)
-              s4[q & 3] = add2(s4[q & 3], pk(ex2(f[2 * q]), ex2(f[2 * q + 1])));
           }
-          float a0, a1;
-          upk(add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])), a0, a1);
-          sum += a0 + a1;
+          if (!seen && gm != -INFINITY) {
+            seen = true;
+            base = fabsf(gm) > 64.f && fabsf(gm) < INFINITY ? gm : 0.f;
+          } else if (gm > base + 64.f && gm < INFINITY) {
+            sum *= ex2(base - gm);
+            base = gm;
+          }
+          fresh = __any_sync(~0u, !seen);
+          based = __any_sync(~0u, base != 0.f);
+          const uint64_t nb = pk(-base, -base);
+          uint64_t s4[4] = {0, 0, 0, 0};
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g) {
+            uint32_t v[32];
+            uint64_t y[16];
+            tmem_ld32(ts + 32 * g, v);
+            tmem_ld_wait(v);
+            logits32(y, v, terms + 32 * g);
+            add_exp<true>(s4, y, nb);
+          }
+          add = sum4(s4);
+        }
+        sum += add;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s_empty[b]);
+          mbar_arrive(&c_empty[cs]);
         }
       }
-      // the four column shares of a row into one (max, sum relative to it).
-      // A NaN logit does not show in the maximum but makes the sum NaN.
-      const float rel = my == -INFINITY ? sum : sum * ex2(base - my);
+      const float top = seen ? base : -INFINITY;
+      // the four column shares of a row into one (base, sum relative to it)
       float *cp = comb + (seg & 1) * 8 * kTile;
-      cp[(ew >> 2) * 2 * kTile + r] = my;
-      cp[(ew >> 2) * 2 * kTile + kTile + r] = rel;
+      cp[(ew >> 2) * 2 * kTile + r] = top;
+      cp[(ew >> 2) * 2 * kTile + kTile + r] = sum;
       ok = named_bar_and(1, kEpiThreads, ok);
       if (!ok) break;
       if ((ew >> 2) == 0) {
-        float M = my;
+        float M = top;
 #pragma unroll
         for (int q = 1; q < 4; ++q) M = fmaxf(M, cp[q * 2 * kTile + r]);
         float S = 0.f;
@@ -618,29 +730,82 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
   }
 }
 
-// Joins the pieces of every kept row, in the order of the vocabulary.
-__global__ void __launch_bounds__(128)
-ce_loss_kernel(const Header *hdr, const int *rowidx, const float *lt, const float2 *part,
-               int chunks, int G, float *loss, float *lse) {
-  const int n = hdr->n;
-  const int tile = blockIdx.x, r = threadIdx.x;
-  const int row = tile * kTile + r;
-  if (row >= n) return;
-  const long long total = (long long)((n + kTile - 1) / kTile) * chunks;
-  const int ca = owner(total, (long long)tile * chunks, G);
-  const int cb = owner(total, (long long)(tile + 1) * chunks - 1, G);
+// sum of products of two rows of K 16-bit numbers, over the lanes of a warp
+template <bool BF16>
+__device__ __forceinline__ float warp_dot(const uint8_t *a, const uint8_t *b, int K, int lane) {
+  float s = 0.f;
+  if (8 * lane < K) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(a) + lane);
+    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(b) + lane);
+    const uint32_t x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float2 f, g;
+      if (BF16) {
+        f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&x[k]));
+        g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&y[k]));
+      } else {
+        f = __half22float2(*reinterpret_cast<const __half2 *>(&x[k]));
+        g = __half22float2(*reinterpret_cast<const __half2 *>(&y[k]));
+      }
+      s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  return s;
+}
+
+// Joins the pieces of every kept row, in the order of the vocabulary: a CTA
+// takes 32 rows of a tile, eight threads per row a run of its pieces each. The
+// target's logit is a dot product here: picking it out of the tiles would cost
+// every tile a search.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+ce_loss_kernel(const FwdParams p, const uint8_t *w, const float *bias, const int *tgt, int grid,
+               float *loss, float *lse) {
+  __shared__ int s_first, s_last;
+  __shared__ float2 s_run[8][32];
+  __shared__ float s_lt[32];
+  const int n = p.hdr->n;
+  const int tile = blockIdx.x / (kTile / 32), r0 = blockIdx.x % (kTile / 32) * 32;
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int row0 = tile * kTile + r0;
+  if (row0 >= n) return;
+  if (threadIdx.x == 0) {
+    const Cuts cuts((long long)((n + kTile - 1) / kTile) * p.chunks, grid);
+    s_first = cuts.owner((long long)tile * p.chunks);
+    s_last = cuts.owner((long long)(tile + 1) * p.chunks - 1);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int row = row0 + run * 4 + k;
+    if (row >= n) break;
+    const int t = tgt[row];
+    const float d = warp_dot<BF16>(p.feat + (size_t)p.rowidx[row] * p.K * 2,
+                                   w + (size_t)t * p.K * 2, p.K, lane);
+    if (lane == 0) s_lt[run * 4 + k] = d + (bias ? bias[t] : 0.f);
+  }
+  __syncthreads();
+  const int pieces = s_last - s_first + 1, per = (pieces + 7) / 8;
   float M = -INFINITY, S = 0.f;
-  for (int c = ca; c <= cb; ++c) {
-    if (cut(total, c, G) == cut(total, c + 1, G)) continue;
-    const float2 v = part[(size_t)(tile + c) * kTile + r];
+  auto join = [&](float2 v) {  // a NaN shows in the sums only
     const float m = fmaxf(M, v.x);
     S = (M == -INFINITY ? S : S * exp2f(M - m)) + (v.x == -INFINITY ? v.y : v.y * exp2f(v.x - m));
     M = m;
-  }
-  const float ls = logf(S);
-  const int i = rowidx[row];
-  lse[i] = fmaf(M, kLn2, ls);
-  loss[i] = fmaf(M - lt[row], kLn2, ls);
+  };
+  const float2 *src = p.part + (size_t)(tile + s_first) * kTile + r0 + lane;
+#pragma unroll 4
+  for (int c = run * per; c < min(pieces, (run + 1) * per); ++c) join(src[(size_t)c * kTile]);
+  s_run[run][lane] = make_float2(M, S);
+  __syncthreads();
+  if (run > 0 || row0 + lane >= n) return;
+  for (int k = 1; k < 8; ++k) join(s_run[k][lane]);
+  const float z = fmaf(M, kLn2, logf(S));
+  const float l = z - s_lt[lane];
+  const int i = p.rowidx[row0 + lane];
+  lse[i] = z;
+  loss[i] = l < 0.f ? 0.f : l;  // a sum is its own term at least; keeps NaN
 }
 
 // ------------------------------------------------------------- backward -----
@@ -648,23 +813,24 @@ template <int KA>
 struct BwdCfg {
   static constexpr int KP = 64 * KA;
   static constexpr int CN = KA <= 2 ? 128 : 64;       // streamed rows of a chunk
-  static constexpr int HC = CN / 2;                   // columns of S per epilogue warp
+  static constexpr int QC = CN / 4;                   // columns of S per epilogue warp
   static constexpr int STAGE = KP * CN * 2;
   static constexpr int STAGES = KA == 1 ? 8 : KA == 2 ? 5 : KA == 3 ? 7 : 5;
   static constexpr int TD = 0, TX = KP, TS = KP + KP / 2;  // TMEM columns: D, tile, two S
-  static constexpr int OFF_BAR = STAGES * STAGE;
-  static constexpr int NBAR = 2 * STAGES + 6;
+  static constexpr int COL = 3 * CN * 4;              // addend, scale and target of each row
+  static constexpr int OFF_COL = STAGES * STAGE;
+  static constexpr int OFF_BSUM = OFF_COL + kColSlots * COL;        // [2][4][128] floats
+  static constexpr int OFF_BAR = OFF_BSUM + 2 * 4 * kTile * 4;
+  static constexpr int NBAR = 2 * STAGES + 2 * kColSlots + 6;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-  static constexpr int OFF_BSUM = (OFF_MISC + 16 + 15) / 16 * 16;   // [2][4][128] floats
-  static constexpr int OFF_COL = OFF_BSUM + 2 * 4 * kTile * 4;      // [16][3][32] words
-  static constexpr int SMEM = OFF_COL + kEpiWarps * 96 * 4 + 1024;
+  static constexpr int SMEM = OFF_MISC + 16 + 1024;
   static_assert(TS + 2 * CN <= kTmemCols, "tensor memory");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 struct BwdParams {
   const uint8_t *w, *xc;
-  const float *bias;
+  const float *bias2;
   const Header *hdr;
   const int *rowidx, *tgt;
   const float *nlse, *gc, *gs;
@@ -717,10 +883,11 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
   uint64_t *p_full = s_full + 2;            // [2]
   uint64_t *x_ready = p_full + 2;
   uint64_t *d_full = x_ready + 1;
+  uint64_t *c_full = d_full + 1;
+  uint64_t *c_empty = c_full + kColSlots;
   uint32_t *s_tmem = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
   volatile int *s_abort = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 4);
   float *bsum = reinterpret_cast<float *>(smem + C::OFF_BSUM);
-  float *scol = reinterpret_cast<float *>(smem + C::OFF_COL);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -730,7 +897,11 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&p_full[b], kEpiWarps / 2);
+      mbar_init(&p_full[b], kEpiWarps);
+    }
+    for (int b = 0; b < kColSlots; ++b) {
+      mbar_init(&c_full[b], 1);
+      mbar_init(&c_empty[b], kEpiWarps);
     }
     mbar_init(x_ready, kEpiWarps);
     mbar_init(d_full, 1);
@@ -746,49 +917,76 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
   const BwdLine line(p.hdr, C::CN, p.chunks_v, p.want_x, p.tiles_w);
-  const long long it0 = cut(line.total, blockIdx.x, gridDim.x);
-  const long long it1 = cut(line.total, blockIdx.x + 1, gridDim.x);
+  const Cuts cuts(line.total, gridDim.x);
+  const long long it0 = cuts.at(blockIdx.x), it1 = cuts.at(blockIdx.x + 1);
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       tma_prefetch_desc(&wmap);
       tma_prefetch_desc(&xmap);
-      long long j = 0;
-      for (long long it = it0; it < it1; ++it, ++j) {
-        const int s = (int)(j % C::STAGES);
-        const uint32_t u = (uint32_t)(j / C::STAGES);
-        if (u > 0 && !mbar_wait_bounded(&b_empty[s], (u - 1) & 1, s_abort, p.err, 71)) break;
-        mbar_arrive_expect_tx(&b_full[s], C::STAGE);
+      Ring<C::STAGES> bs;
+      Ring<kColSlots> cr;
+      bool ok = true;
+      for (long long it = it0; ok && it < it1;) {
         bool dw;
-        int tile, c, nc;
-        line.at(it, dw, tile, c, nc);
-        for (int k = 0; k < KA; ++k)
-          tma_load_2d(smem + s * C::STAGE + k * C::CN * 128, dw ? &xmap : &wmap, &b_full[s], 64 * k,
-                      c * C::CN);
+        int tile, c0, nc;
+        line.at(it, dw, tile, c0, nc);
+        const int cnt = (int)min((long long)(nc - c0), it1 - it);
+        it += cnt;
+        const CUtensorMap *map = dw ? &xmap : &wmap;
+        for (int c = c0; c < c0 + cnt; ++c) {
+          ok = bs.first || mbar_wait_bounded(&b_empty[bs.i], bs.phase ^ 1, s_abort, p.err, 71);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&b_full[bs.i], C::STAGE);
+          uint8_t *dst = smem + bs.i * C::STAGE;
+#pragma unroll
+          for (int k = 0; k < KA; ++k)
+            tma_load_2d(dst + k * C::CN * 128, map, &b_full[bs.i], 64 * k, c * C::CN);
+          bs.next();
+          ok = cr.first || mbar_wait_bounded(&c_empty[cr.i], cr.phase ^ 1, s_abort, p.err, 77);
+          if (!ok) break;
+          uint8_t *col = smem + C::OFF_COL + cr.i * C::COL;
+          const size_t at = (size_t)c * C::CN;
+          mbar_arrive_expect_tx(&c_full[cr.i], dw ? C::COL : C::CN * 4);
+          if (dw) {
+            bulk_load(col, p.nlse + at, C::CN * 4, &c_full[cr.i]);
+            bulk_load(col + C::CN * 4, p.gs + at, C::CN * 4, &c_full[cr.i]);
+            bulk_load(col + 2 * C::CN * 4, p.tgt + at, C::CN * 4, &c_full[cr.i]);
+          } else {
+            bulk_load(col, p.bias2 + at, C::CN * 4, &c_full[cr.i]);
+          }
+          cr.next();
+        }
       }
-      if (*s_abort) drain_loads(b_full, j, C::STAGES);
+      if (*s_abort) {
+        drain_loads(b_full, bs);
+        drain_loads(c_full, cr);
+      }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t id1 = BF16 ? idesc_bf16(kTile, C::CN) : idesc_f16(kTile, C::CN);
       constexpr uint32_t id2 =
           (BF16 ? idesc_bf16(kTile, C::KP) : idesc_f16(kTile, C::KP)) | kIdescBMnMajor;
-      long long j = 0;  // chunk of this CTA
+      const uint64_t kdesc = sw128_kmajor_desc(smem_u32(smem));
+      const uint64_t mdesc = sw128_mnmajor_desc(smem_u32(smem), C::CN * 128);
+      Ring<C::STAGES> b1, b2;  // chunks of the first and of the second product
+      Ring<2> s1, s2;
       uint32_t seg = 0;
       bool ok = true;
-      // S = tile x chunk^T of chunk jj into its buffer
-      auto first = [&](long long jj) {
-        const int s = (int)(jj % C::STAGES);
-        const uint32_t u = (uint32_t)(jj / C::STAGES);
-        if (!mbar_wait_bounded(&b_full[s], u & 1, s_abort, p.err, 72)) return false;
+      // S = tile x chunk^T of the next chunk into its buffer
+      auto first = [&]() {
+        if (!mbar_wait_bounded(&b_full[b1.i], b1.phase, s_abort, p.err, 72)) return false;
         tc_fence_after();
-        const uint32_t baddr = smem_u32(smem + s * C::STAGE);
+        const uint64_t bd = kdesc + (uint64_t)(b1.i * (C::STAGE >> 4));
+        const uint32_t d = tmem + C::TS + s1.i * C::CN;
 #pragma unroll
         for (int k = 0; k < 4 * KA; ++k)
-          mma_f16_ts(tmem + C::TS + (uint32_t)(jj & 1) * C::CN, tmem + C::TX + 8 * k,
-                     sw128_kmajor_desc(baddr + (k >> 2) * (C::CN * 128) + 32u * (k & 3)), id1,
-                     k > 0 ? 1u : 0u);
-        mma_commit(&s_full[jj & 1]);
+          mma_f16_ts(d, tmem + C::TX + 8 * k, bd + (((k >> 2) * (C::CN * 128) + 32 * (k & 3)) >> 4),
+                     id1, k > 0 ? 1u : 0u);
+        mma_commit(&s_full[s1.i]);
+        b1.next();
+        s1.next();
         return true;
       };
       for (long long it = it0; ok && it < it1; ++seg) {
@@ -796,46 +994,43 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         int tile, c0, nc;
         line.at(it, dw, tile, c0, nc);
         const int cnt = (int)min((long long)(nc - c0), it1 - it);
+        it += cnt;
         ok = mbar_wait_bounded(x_ready, seg & 1, s_abort, p.err, 73);
         if (!ok) break;
         tc_fence_after();
-        ok = first(j) && (cnt < 2 || first(j + 1));
-        for (int i = 0; ok && i < cnt; ++i, ++j) {
-          const int s = (int)(j % C::STAGES), b = (int)(j & 1);
-          ok = mbar_wait_bounded(&p_full[b], (uint32_t)(j >> 1) & 1, s_abort, p.err, 74);
+        ok = first() && (cnt < 2 || first());
+        for (int i = 0; ok && i < cnt; ++i) {
+          ok = mbar_wait_bounded(&p_full[s2.i], s2.phase, s_abort, p.err, 74);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t baddr = smem_u32(smem + s * C::STAGE);
+          const uint64_t bd = mdesc + (uint64_t)(b2.i * (C::STAGE >> 4));
+          const uint32_t pa = tmem + C::TS + s2.i * C::CN;
 #pragma unroll
           for (int k = 0; k < C::CN / 16; ++k) {
-            // P of each half of the chunk lies at the head of that half's S columns
-            const uint32_t pc = (16 * k / C::HC) * C::HC + (16 * k % C::HC) / 2;
-            mma_f16_ts(tmem + C::TD, tmem + C::TS + (uint32_t)b * C::CN + pc,
-                       sw128_mnmajor_desc(baddr + 2048u * k, C::CN * 128), id2,
-                       i > 0 || k > 0 ? 1u : 0u);
+            // P of each quarter of the chunk lies at the head of that quarter's S columns
+            const uint32_t pc = (16 * k / C::QC) * C::QC + (16 * k % C::QC) / 2;
+            mma_f16_ts(tmem + C::TD, pa + pc, bd + ((2048 * k) >> 4), id2, i > 0 || k > 0 ? 1u : 0u);
           }
-          mma_commit(&b_empty[s]);
-          if (i + 1 == cnt) mma_commit(d_full);
+          mma_commit(&b_empty[b2.i]);
+          b2.next();
+          s2.next();
           // the next S into this buffer: issued after the product that reads P
           // there, and the tensor pipe keeps that order
-          if (i + 2 < cnt) ok = first(j + 2);
+          if (i + 2 < cnt) ok = first();
+          if (i + 1 == cnt) mma_commit(d_full);
         }
-        it += cnt;
       }
     }
   } else {
     const int ew = warp - kEpiWarp0;
-    const int grp = ew >> 3;
-    const int half = (ew >> 2) & 1;
-    const int w4 = ew >> 2;
+    const int w4 = ew >> 2;              // its quarter of the columns
     const int quad = warp & 3;
     const int r = quad * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16);
-    float *ccol = scol + ew * 96;      // additive term of y per column
-    float *csc = ccol + 32;            // dW: scale per column
-    int *ctg = reinterpret_cast<int *>(ccol + 64);  // dW: target per column
     const uint64_t l2e2 = pk(kLog2e, kLog2e);
-    long long j = 0;
+    constexpr int QC = C::QC;
+    Ring<2> sr;
+    Ring<kColSlots> cr;
     int seg = 0;
     bool ok = true;
     for (long long it = it0; it < it1; ++seg) {
@@ -854,94 +1049,79 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
       // y = S * log2(e) + column term + row term; P = exp2(y) (* column scale)
       const int tg = !dw && real ? p.tgt[row] : -1;
       float rterm = -INFINITY;
-      if (real) rterm = dw ? (p.bias ? p.bias[row] * kLog2e : 0.f) : p.nlse[row] + p.shift;
+      if (real) rterm = dw ? p.bias2[row] : p.nlse[row] + p.shift;
       const uint64_t rt2 = pk(rterm, rterm);
       const float one = exp2f(p.shift);
       uint64_t acc2 = 0;
-      for (int i = 0; i < cnt; ++i, ++j) {
-        const int b = (int)(j & 1);
-        if (b != grp) continue;
-        const int v0 = (c0 + i) * C::CN + half * C::HC;
-        float ct[C::HC / 32], cs[C::HC / 32];
-        int cg[C::HC / 32];
-#pragma unroll
-        for (int g = 0; g < C::HC / 32; ++g) {
-          const int v = v0 + 32 * g + lane;
-          if (dw) {  // the arrays reach to the end of the last tile
-            ct[g] = __ldg(p.nlse + v);
-            cs[g] = __ldg(p.gs + v);
-            cg[g] = __ldg(p.tgt + v);
-          } else {
-            ct[g] = v < p.V ? (p.bias ? __ldg(p.bias + v) * kLog2e : 0.f) : -INFINITY;
-          }
-        }
-        ok = ok && mbar_wait_bounded(&s_full[b], (uint32_t)(j >> 1) & 1, s_abort, p.err, 75);
+      for (int i = 0; i < cnt; ++i, sr.next(), cr.next()) {
+        const int b = sr.i, cs = cr.i;
+        ok = ok && mbar_wait_bounded(&c_full[cs], cr.phase, s_abort, p.err, 78) &&
+             mbar_wait_bounded(&s_full[b], sr.phase, s_abort, p.err, 75);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ts = tl + C::TS + b * C::CN + half * C::HC;
+        const uint32_t ts = tl + C::TS + b * C::CN + w4 * QC;
+        const float *col = reinterpret_cast<const float *>(smem + C::OFF_COL + cs * C::COL) + w4 * QC;
+        uint32_t v[QC];
+        if constexpr (QC == 32)
+          tmem_ld32(ts, v);
+        else
+          tmem_ld16(ts, v);
+        tmem_ld_wait(v);
+        float f[QC];
+        const ulonglong2 *cq = reinterpret_cast<const ulonglong2 *>(col);
 #pragma unroll
-        for (int g = 0; g < C::HC / 32; ++g) {
-          uint32_t v[32];
-          tmem_ld32(ts + 32 * g, v);
-          const int cb = v0 + 32 * g;
-          __syncwarp();
-          ccol[lane] = ct[g];
-          if (dw) {
-            csc[lane] = cs[g];
-            ctg[lane] = cg[g];
-          }
-          __syncwarp();
-          tmem_ld_wait(v);
-          float f[32];
-          const ulonglong2 *cq = reinterpret_cast<const ulonglong2 *>(ccol);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const ulonglong2 bb = cq[q];
-            upk(add2(fma2(pk(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1])), l2e2, bb.x),
-                     rt2),
-                f[4 * q], f[4 * q + 1]);
-            upk(add2(fma2(pk(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])), l2e2,
-                          bb.y),
-                     rt2),
-                f[4 * q + 2], f[4 * q + 3]);
-          }
-#pragma unroll
-          for (int q = 0; q < 32; ++q) f[q] = ex2(f[q]);
-          if (dw) {
-            // columns whose target is among this warp's 32 classes
-            const int v32 = tile * kTile + quad * 32;
-            const bool any = __any_sync(~0u, cg[g] >= v32 && cg[g] < v32 + 32);
-            if (any) {
-#pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (ctg[q] == row) f[q] -= 1.f;
-            }
-            const ulonglong2 *sq = reinterpret_cast<const ulonglong2 *>(csc);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const ulonglong2 ss = sq[q];
-              const uint64_t a = mul2(pk(f[4 * q], f[4 * q + 1]), ss.x);
-              const uint64_t c = mul2(pk(f[4 * q + 2], f[4 * q + 3]), ss.y);
-              acc2 = add2(acc2, add2(a, c));
-              upk(a, f[4 * q], f[4 * q + 1]);
-              upk(c, f[4 * q + 2], f[4 * q + 3]);
-            }
-          } else {
-            if (__any_sync(~0u, tg >= cb && tg < cb + 32)) {
-#pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (tg == cb + q) f[q] -= one;
-            }
-          }
-          uint32_t h[16];
-#pragma unroll
-          for (int q = 0; q < 16; ++q) h[q] = pack16<BF16>(f[2 * q], f[2 * q + 1]);
-          tmem_st16(ts + 16 * g, h);
+        for (int q = 0; q < QC / 4; ++q) {
+          const ulonglong2 bb = cq[q];
+          upk(add2(fma2(pk(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1])), l2e2, bb.x),
+                   rt2),
+              f[4 * q], f[4 * q + 1]);
+          upk(add2(fma2(pk(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])), l2e2, bb.y),
+                   rt2),
+              f[4 * q + 2], f[4 * q + 3]);
         }
+#pragma unroll
+        for (int q = 0; q < QC; ++q) f[q] = ex2(f[q]);
+        if (dw) {
+          // columns whose target is among this warp's 32 classes
+          const int *ctg = reinterpret_cast<const int *>(col + 2 * C::CN);
+          const int off = ctg[lane % QC] - (tile * kTile + quad * 32);
+          if (__any_sync(~0u, off >= 0 && off < 32)) {
+#pragma unroll
+            for (int q = 0; q < QC; ++q)
+              if (ctg[q] == row) f[q] -= 1.f;
+          }
+          const ulonglong2 *sq = reinterpret_cast<const ulonglong2 *>(col + C::CN);
+#pragma unroll
+          for (int q = 0; q < QC / 4; ++q) {
+            const ulonglong2 ss = sq[q];
+            const uint64_t a = mul2(pk(f[4 * q], f[4 * q + 1]), ss.x);
+            const uint64_t c = mul2(pk(f[4 * q + 2], f[4 * q + 3]), ss.y);
+            acc2 = add2(acc2, add2(a, c));
+            upk(a, f[4 * q], f[4 * q + 1]);
+            upk(c, f[4 * q + 2], f[4 * q + 3]);
+          }
+        } else {
+          const int at = tg - ((c0 + i) * C::CN + w4 * QC);
+          if (__any_sync(~0u, at >= 0 && at < QC)) {
+#pragma unroll
+            for (int q = 0; q < QC; ++q)
+              if (at == q) f[q] -= one;
+          }
+        }
+        uint32_t h[QC / 2];
+#pragma unroll
+        for (int q = 0; q < QC / 2; ++q) h[q] = pack16<BF16>(f[2 * q], f[2 * q + 1]);
+        if constexpr (QC == 32)
+          tmem_st16(ts, h);
+        else
+          tmem_st8(ts, h);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
+        if (lane == 0) {
+          mbar_arrive(&p_full[b]);
+          mbar_arrive(&c_empty[cs]);
+        }
       }
       float a0, a1;
       upk(acc2, a0, a1);
@@ -1013,53 +1193,62 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
 // border (CTA c > 0), y: a slice of the tile.
 template <bool BF16>
 __global__ void __launch_bounds__(256)
-ce_join_kernel(const BwdParams p, int cn, int KP, int G) {
-  const BwdLine line(p.hdr, cn, p.chunks_v, p.want_x, p.tiles_w);
-  // the first border inside a tile handles that tile (with few steps some
-  // CTAs have an empty range)
-  const int c = blockIdx.x + 1;
-  const long long at = cut(line.total, c, G);
-  if (at == 0 || at == cut(line.total, c + 1, G)) return;
-  bool dw;
-  int tile, chunk, nc;
-  line.at(at, dw, tile, chunk, nc);
-  if (chunk == 0) return;
-  const long long t0 = at - chunk;  // first step of the tile
-  const int head = owner(line.total, at - 1, G);
-  if (cut(line.total, head, G) > t0) return;
-  int last = c;
-  while (last + 1 < G && cut(line.total, last + 1, G) < t0 + nc) ++last;
-  const int lim = min(kTile, (dw ? p.V : line.n) - tile * kTile);
+ce_join_kernel(const BwdParams p, int cn, int KP, int grid) {
+  __shared__ int s_tile, s_dw, s_last;
+  if (threadIdx.x == 0) {
+    s_tile = -1;
+    const BwdLine line(p.hdr, cn, p.chunks_v, p.want_x, p.tiles_w);
+    const Cuts cuts(line.total, grid);
+    const int c = blockIdx.x + 1;
+    if (c < cuts.G) {
+      const long long at = cuts.at(c);
+      bool dw;
+      int tile, chunk, nc;
+      line.at(at, dw, tile, chunk, nc);
+      const long long t0 = at - chunk;  // first step of the tile
+      // the first border inside a tile handles that tile
+      if (chunk > 0 && cuts.at(c - 1) <= t0) {
+        s_tile = tile;
+        s_dw = dw;
+        s_last = cuts.owner(t0 + nc - 1);
+      }
+    }
+  }
+  __syncthreads();
+  const int tile = s_tile;
+  if (tile < 0) return;
+  const bool dw = s_dw;
+  const int c = blockIdx.x + 1, last = s_last;  // pieces: the tail of CTA c - 1, then c .. last
+  const int lim = min(kTile, (dw ? p.V : p.hdr->n) - tile * kTile);
   const int q4 = KP / 4;
   const float gmax = p.hdr->gmax;
   const int step = gridDim.y * blockDim.x;
-  for (int e = blockIdx.y * blockDim.x + threadIdx.x; e < lim * q4; e += step) {
-    const int r = e / q4, k = (e - r * q4) * 4;
-    if (k >= p.K || (dw && !p.dw)) continue;
-    const size_t o = (size_t)r * KP + k;
-    const float *src = p.dpart + o;
-    const size_t ps = (size_t)kTile * KP;
-    float4 s = *reinterpret_cast<const float4 *>(src + (2 * head + 1) * ps);
-    for (int d = c; d <= last; ++d) {
-      if (cut(line.total, d, G) == cut(line.total, d + 1, G)) continue;
-      const float4 v = *reinterpret_cast<const float4 *>(src + 2 * d * ps);
-      s.x += v.x;
-      s.y += v.y;
-      s.z += v.z;
-      s.w += v.w;
+  const size_t ps = (size_t)kTile * KP;
+  if (!dw || p.dw)
+    for (int e = blockIdx.y * blockDim.x + threadIdx.x; e < lim * q4; e += step) {
+      const int r = e / q4, k = (e - r * q4) * 4;
+      if (k >= p.K) continue;
+      const float *src = p.dpart + (size_t)r * KP + k;
+      float4 s = *reinterpret_cast<const float4 *>(src + (size_t)(2 * c - 1) * ps);
+#pragma unroll 4
+      for (int d = c; d <= last; ++d) {
+        const float4 v = *reinterpret_cast<const float4 *>(src + 2 * (size_t)d * ps);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+      }
+      const int row = tile * kTile + r;
+      const float sc = (dw ? gmax : p.gc[row]) * p.unscale;
+      uint8_t *out = dw ? p.dw + (size_t)row * p.K * 2 : p.dfeat + (size_t)p.rowidx[row] * p.K * 2;
+      *reinterpret_cast<uint2 *>(out + 2 * k) =
+          make_uint2(pack16<BF16>(s.x * sc, s.y * sc), pack16<BF16>(s.z * sc, s.w * sc));
     }
-    const int row = tile * kTile + r;
-    const float sc = (dw ? gmax : p.gc[row]) * p.unscale;
-    const uint2 h = make_uint2(pack16<BF16>(s.x * sc, s.y * sc), pack16<BF16>(s.z * sc, s.w * sc));
-    uint8_t *out = dw ? p.dw + (size_t)row * p.K * 2 : p.dfeat + (size_t)p.rowidx[row] * p.K * 2;
-    *reinterpret_cast<uint2 *>(out + 2 * k) = h;
-  }
   if (dw && p.dbias && blockIdx.y == 0)
     for (int r = threadIdx.x; r < lim; r += blockDim.x) {
-      float s = p.bpart[(size_t)(2 * head + 1) * kTile + r];
-      for (int d = c; d <= last; ++d)
-        if (cut(line.total, d, G) != cut(line.total, d + 1, G))
-          s += p.bpart[(size_t)2 * d * kTile + r];
+      float s = p.bpart[(size_t)(2 * c - 1) * kTile + r];
+#pragma unroll 4
+      for (int d = c; d <= last; ++d) s += p.bpart[(size_t)2 * d * kTile + r];
       p.dbias[tile * kTile + r] = s * (gmax * p.unscale);
     }
 }
@@ -1112,19 +1301,25 @@ int launch_bwd(const BwdParams &p, int rows_pad, int grid, cudaStream_t st) {
 
 template <bool BWD>
 int launch_place(const Workspace &ws, const void *targets, bool wide, int rows, int V, int K,
-                 int dtype, const void *feat, const float *lse, const float *g, void *dfeat,
-                 float *loss, float *lse_out, cudaStream_t st) {
+                 int dtype, const float *bias, const void *feat, const float *lse,
+                 const float *g, void *dfeat, float *loss, float *lse_out, cudaStream_t st) {
   const int blocks = rows > kRowBlock ? (rows + kRowBlock - 1) / kRowBlock : 1;
-  ce_count_kernel<<<blocks, kRowBlock, 0, st>>>(targets, wide, rows, V, g, ws.cnt, ws.gblk);
-  int rc = check_launch("ce_count_kernel");
-  if (rc) return rc;
+  const bool direct = blocks <= kDirect;
+  if (!direct) {
+    ce_count_kernel<<<blocks, kRowBlock, 0, st>>>(targets, wide, rows, V, g, ws.cnt, ws.gblk);
+    const int rc = check_launch("ce_count_kernel");
+    if (rc) return rc;
+  }
   PlaceParams p{};
+  p.direct = direct;
   p.targets = targets;
   p.wide = wide;
   p.rows = rows;
   p.V = V;
   p.K = K;
   p.shift = dtype == TOCR_DTYPE_F16 ? (float)(1 << kShift) : 1.f;
+  p.bias = bias;
+  p.bias2 = ws.bias2;
   p.cnt = ws.cnt;
   p.gblk = ws.gblk;
   p.hdr = ws.hdr;
@@ -1140,7 +1335,7 @@ int launch_place(const Workspace &ws, const void *targets, bool wide, int rows, 
   p.nlse = ws.nlse;
   p.gc = ws.gc;
   p.gs = ws.gs;
-  ce_place_kernel<BWD><<<blocks, kRowBlock, 0, st>>>(p);
+  ce_place_kernel<BWD><<<dim3(blocks, 8), kRowBlock, 0, st>>>(p);
   return check_launch("ce_place_kernel");
 }
 
@@ -1164,7 +1359,7 @@ extern "C" {
 TOCR_API size_t tocr_rec_head_ce_workspace_bytes(long long rows, int K, int num_classes,
                                                  int backward) {
   if (rows < 0 || rows > kMaxRows || K < 8 || K > kMaxK || K % 8 || num_classes <= 0) return 0;
-  return carve(nullptr, rows, K, backward != 0).bytes;
+  return carve(nullptr, rows, K, num_classes, backward != 0).bytes;
 }
 
 TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *d_bias,
@@ -1180,21 +1375,19 @@ TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *
   TOCR_REQUIRE(aligned(d_feat, 16) && aligned(d_w, 16),
                "tocr_rec_head_ce: features and weights must be 16-byte aligned");
   TOCR_REQUIRE(aligned(d_workspace, 256) &&
-                   workspace_bytes >= carve(nullptr, rows, K, false).bytes,
+                   workspace_bytes >= carve(nullptr, rows, K, num_classes, false).bytes,
                "tocr_rec_head_ce: the workspace must be 256-byte aligned and hold %zu bytes",
-               carve(nullptr, rows, K, false).bytes);
+               carve(nullptr, rows, K, num_classes, false).bytes);
   cudaStream_t st = as_stream(stream);
-  const Workspace ws = carve(static_cast<uint8_t *>(d_workspace), rows, K, false);
+  const Workspace ws = carve(static_cast<uint8_t *>(d_workspace), rows, K, num_classes, false);
   rc = launch_place<false>(ws, d_targets, targets_i64 != 0, (int)rows, num_classes, K, dtype,
-                           nullptr, nullptr, nullptr, nullptr, d_loss, d_lse, st);
+                           d_bias, nullptr, nullptr, nullptr, nullptr, d_loss, d_lse, st);
   if (rc) return rc;
   FwdParams p{};
   p.feat = static_cast<const uint8_t *>(d_feat);
-  p.bias = d_bias;
+  p.bias2 = ws.bias2;
   p.hdr = ws.hdr;
   p.rowidx = ws.rowidx;
-  p.tgt = ws.tgt;
-  p.lt = ws.lt;
   p.part = ws.part;
   p.V = num_classes;
   p.K = K;
@@ -1210,8 +1403,8 @@ TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *
     default: rc = bf ? launch_fwd<4, true>(p, d_w, grid, st) : launch_fwd<4, false>(p, d_w, grid, st);
   }
   if (rc) return rc;
-  ce_loss_kernel<<<tiles, kTile, 0, st>>>(ws.hdr, ws.rowidx, ws.lt, ws.part, p.chunks, grid, d_loss,
-                                          d_lse);
+  (bf ? ce_loss_kernel<true> : ce_loss_kernel<false>)<<<tiles * (kTile / 32), 256, 0, st>>>(
+      p, static_cast<const uint8_t *>(d_w), d_bias, ws.tgt, grid, d_loss, d_lse);
   return check_launch("ce_loss_kernel");
 }
 
@@ -1232,20 +1425,20 @@ TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, cons
   TOCR_REQUIRE(aligned(d_feat, 16) && aligned(d_w, 16) && aligned(d_dfeat, 16) && aligned(d_dw, 16),
                "tocr_rec_head_ce_backward: features, weights and their gradients must be 16-byte "
                "aligned");
-  TOCR_REQUIRE(aligned(d_workspace, 256) && workspace_bytes >= carve(nullptr, rows, K, true).bytes,
+  TOCR_REQUIRE(aligned(d_workspace, 256) && workspace_bytes >= carve(nullptr, rows, K, num_classes, true).bytes,
                "tocr_rec_head_ce_backward: the workspace must be 256-byte aligned and hold %zu bytes",
-               carve(nullptr, rows, K, true).bytes);
+               carve(nullptr, rows, K, num_classes, true).bytes);
   cudaStream_t st = as_stream(stream);
-  const Workspace ws = carve(static_cast<uint8_t *>(d_workspace), rows, K, true);
-  rc = launch_place<true>(ws, d_targets, targets_i64 != 0, (int)rows, num_classes, K, dtype, d_feat,
-                          d_lse, d_grad_loss, d_dfeat, nullptr, nullptr, st);
+  const Workspace ws = carve(static_cast<uint8_t *>(d_workspace), rows, K, num_classes, true);
+  rc = launch_place<true>(ws, d_targets, targets_i64 != 0, (int)rows, num_classes, K, dtype, d_bias,
+                          d_feat, d_lse, d_grad_loss, d_dfeat, nullptr, nullptr, st);
   if (rc) return rc;
   const int KA = (K + 63) / 64;
   const int cn = KA <= 2 ? 128 : 64;
   BwdParams p{};
   p.w = static_cast<const uint8_t *>(d_w);
   p.xc = ws.xc;
-  p.bias = d_bias;
+  p.bias2 = ws.bias2;
   p.hdr = ws.hdr;
   p.rowidx = ws.rowidx;
   p.tgt = ws.tgt;

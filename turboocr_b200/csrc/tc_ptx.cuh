@@ -41,6 +41,36 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
   return ok != 0;
 }
 
+// A position in a ring of N slots: slot index, and the parity of the phase that
+// completes when the slot is filled (the emptying phase of its previous use has
+// the other parity; on the first round there is none to wait for). Kept step by
+// step: divisions would cost the single thread that feeds a tensor core more
+// than the MMAs of a chunk.
+template <int N>
+struct Ring {
+  int i = 0;
+  uint32_t phase = 0;
+  bool first = true;
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
+      phase ^= 1;
+      first = false;
+    }
+  }
+};
+
+// True in one lane of a converged warp. Unlike a test of the lane number it
+// tells the compiler that one thread runs the branch, so MMA descriptors stay in
+// uniform registers without a loop over the active lanes around each MMA.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // Bounded wait: spins on try_wait until the phase with `parity` completes,
 // the shared abort flag is raised by another role, or ~2^31 cycles pass.
 // Returns false on timeout/abort (the caller then unwinds); on timeout the
@@ -104,6 +134,16 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *m, uin
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+// `bytes` (a multiple of 16) of consecutive memory, both addresses on 16 bytes.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes,
+                                          uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
 
