@@ -80,3 +80,40 @@ def test_linear(tocr, cuda, rows, K, N, xt, yt):
     act = ["none", "relu", "hardswish"][(rows + K + N) % 3]
     err = torch.zeros(1, dtype=torch.int32, device=cuda)
     check(x, w, bias, act, yt, err)
+
+
+@pytest.mark.parametrize("rows,K,N,out", [(2100, 40, 18385, F16), (1000, 33, 18387, F32),
+                                          (8400, 300, 4099, BF16), (37, 16, 1000003, F16),
+                                          (70001, 16, 500, F16)])
+def test_outputs_larger_than_l2(tocr, cuda, rows, K, N, out):
+    """Outputs of more than 64 MB whose rows are not sector-aligned take their
+    own way out of the kernel."""
+    g = torch.Generator(device="cpu").manual_seed(rows)
+    x = torch.randn(rows, K, generator=g).half().to(cuda)
+    w = (torch.randn(N, K, generator=g) / math.sqrt(K)).to(cuda)
+    bias = torch.randn(N, generator=g).to(cuda)
+    check(x, w, bias, "none", out, torch.zeros(1, dtype=torch.int32, device=cuda))
+
+
+@pytest.mark.parametrize("rows,N,out", [(2100, 18385, F16), (2100, 18384, BF16), (130, 77, F16),
+                                        (1100, 16385, F32)])
+def test_output_at_any_element_and_nothing_written_around_it(tocr, cuda, rows, N, out):
+    K, pad = 48, 67
+    g = torch.Generator(device="cpu").manual_seed(N)
+    x = torch.randn(rows, K, generator=g).half().to(cuda)
+    w = torch.randn(N, K, generator=g).to(cuda)
+    wq, ws = linear_i8.quantize_rows(w)
+    xq, sx = linear_i8.quantize_rows(x)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    want = linear_i8.linear_codes(xq, sx, K, wq, ws, None, out_dtype=out, err=err)
+    for off in (0, 1, 3, 8):
+        buf = torch.full((pad + off + rows * N + pad,), -7.0, dtype=out, device=cuda)
+        at = buf.data_ptr() + (pad + off) * buf.element_size()
+        st = tocr.lib().tocr_linear_i8_codes(
+            xq.data_ptr(), sx.data_ptr(), rows, K, wq.data_ptr(), ws.data_ptr(), None, N, 0,
+            {F16: 0, BF16: 1, F32: 2}[out], at, err.data_ptr(),
+            torch.cuda.current_stream().cuda_stream)
+        assert st == 0
+        assert torch.equal(buf[pad + off:pad + off + rows * N].view(rows, N), want), off
+        assert bool((buf[:pad + off] == -7).all()) and bool((buf[pad + off + rows * N:] == -7).all())
+    assert int(err) == 0

@@ -14,15 +14,16 @@
 // Quantiser: one pass over x from memory (a row's values stay in registers
 // between its maximum and its codes); bound by HBM.
 //
-// Product: one persistent CTA per SM. Warp 0 loads 128 x 128-byte tiles of
-// the token codes and BN x 128-byte tiles of the weight codes by TMA (128-byte
-// swizzle) into a ring, one thread of warp 1 issues tcgen05.mma kind::i8
-// (M 128, N = BN, K 32) into one of two TMEM accumulators, eight epilogue warps
-// read the other, scale, add the bias, apply the activation and write the rows
-// out through shared memory (a row piece of 128 bytes per store instruction,
-// whatever the alignment of y's rows: the dictionary's 18385 columns leave
-// every other row on an odd 2-byte boundary, where TMA cannot store). BN is
-// 256, or 128 or 64 where larger tiles would leave SMs idle.
+// Product: the output channels are the rows of the MMA (M 128, the lanes of
+// tensor memory) and the tokens its columns (N = BT, 16 to 256), so a thread of
+// the epilogue keeps its channel's scale and bias in registers, and a warp
+// stores 32 neighbouring channels of one token with one instruction straight
+// from registers, whatever the alignment of y's rows (the dictionary's 18385
+// columns leave most of them off every boundary). One persistent CTA per SM:
+// warp 0 loads 128 x 128-byte tiles of the weight codes and BT x 128-byte tiles
+// of the token codes by TMA (128-byte swizzle) into a ring, one thread of warp 1
+// issues tcgen05.mma kind::i8 into one of two TMEM accumulators, and sixteen
+// warps run the epilogue of the other.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,6 +31,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "tc_ptx.cuh"
 #include "tma_map.cuh"
@@ -222,121 +224,113 @@ int quant_rows(const void *x, int dtype, long long rows, int K, int8_t *q, float
 }
 
 // ----------------------------------------------------------------- product --
-constexpr int kBM = 128;
-constexpr int kEpiWarp0 = 2, kEpiWarps = 8;
+constexpr int kBM = 128;         // channels of a tile
+constexpr int kMaxBT = 256;      // tokens of a tile, a multiple of 16
+constexpr int kUnit = 16;        // tokens an epilogue warp takes at a time
+constexpr int kMaxStages = 10;
+constexpr int kEpiWarp0 = 2, kEpiWarps = 16;
 constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
-constexpr int kPitchW = 36;  // words of a staged row piece: 32, and 4 against bank conflicts
-
-template <int BN>
-struct Cfg {
-  static constexpr int STAGE_A = kBM * 128, STAGE_B = BN * 128;
-  static constexpr int STAGE = STAGE_A + STAGE_B;
-  static constexpr int STAGES = BN == 256 ? 3 : BN == 128 ? 5 : 7;
-  static constexpr int OFF_BAR = STAGES * STAGE;
-  static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 4) * 8;
-  static constexpr int OFF_STG = (OFF_MISC + 16 + 15) / 16 * 16;
-  static constexpr int OFF_COL = OFF_STG + kEpiWarps * 32 * kPitchW * 4;
-  static constexpr int SMEM = OFF_COL + kEpiWarps * 64 * 8 + 1024;
-  static constexpr int TMEM = 2 * BN;
-  static_assert(SMEM <= 227 * 1024, "shared memory");
-};
+constexpr int kStageA = kBM * 128;
+constexpr int kOffSx = 0;                                 // [warps][2][64] token scales
+constexpr int kOffBar = kOffSx + kEpiWarps * 2 * 64 * 4;
+constexpr int kOffMisc = kOffBar + (2 * kMaxStages + 4) * 8;
+constexpr int kOffRing = (kOffMisc + 16 + 1023) / 1024 * 1024;
+constexpr int kSmem = 226 * 1024;
+constexpr int kRingBytes = kSmem - 1024 - kOffRing;
 
 struct LinParams {
   const float *sx, *sw, *bias;
   void *y;
   long long rows;
-  int N, ksteps, K;
-  long long tiles_n, tiles;
+  int N, ksteps;
+  int bt, stages;                // tokens of a tile, slots of the ring
+  int tiles_n;
+  long long tiles;
   int act;
-  bool vec;          // rows of y start on 16-byte boundaries
   int *err;
 };
 
-// One 32-row piece of y (32 words per row at most, PC columns from `col` on,
-// clipped at N), staged by the calling warp at stg (row pitch kPitchW words),
-// to global memory. vec: every row of y starts on a 16-byte boundary.
-template <typename T, int PC>
-__device__ __forceinline__ void write_piece(T *y, long long row0, long long rows, int N, int col,
-                                            bool vec, const uint32_t *stg, int lane) {
-  constexpr int PER = 4 / sizeof(T);      // elements per word
-  constexpr int W = PC / PER;             // words of a row
-  const int n = min(N - col, PC);         // elements of a row
-  const int nr = (int)min((long long)32, rows - row0);
-  T *o = y + row0 * N + col;
-  if (vec && n == PC) {
-    constexpr int LPR = W / 4, RPI = 32 / LPR;  // lanes per row, rows per instruction
-    const int r = lane / LPR, w = lane % LPR * 4;
-#pragma unroll 8
-    for (int r0 = 0; r0 < 32; r0 += RPI)
-      if (r0 + r < nr)
-        *reinterpret_cast<uint4 *>(reinterpret_cast<uint32_t *>(o + (long long)(r0 + r) * N) + w) =
-            *reinterpret_cast<const uint4 *>(stg + (r0 + r) * kPitchW + w);
-  } else if constexpr (PER == 1) {
-    if (lane < n)
-#pragma unroll 8
-      for (int r = 0; r < 32; ++r)
-        if (r < nr) reinterpret_cast<uint32_t *>(o + (long long)r * N)[lane] = stg[r * kPitchW + lane];
+__device__ __forceinline__ float activate(float y, int act) {
+  if (act == TOCR_ACT_RELU) return y < 0.f ? 0.f : y;  // keeps NaN
+  return y * (fminf(fmaxf(y + 3.f, 0.f), 6.f) * (1.f / 6.f));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __half>)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// f[j] to token j's row: g, g + ld, ... for the first n of 16 tokens
+template <typename T, bool FULL>
+__device__ __forceinline__ void store_unit(T *g, long long ld, const float (&f)[kUnit], int n) {
+  if constexpr (sizeof(T) == 2) {
+    uint16_t *o = reinterpret_cast<uint16_t *>(g);
+#pragma unroll
+    for (int j = 0; j < kUnit; j += 2) {
+      const uint32_t w = pack2<T>(f[j], f[j + 1]);
+      if (FULL || j < n) o[0] = (uint16_t)w;
+      if (FULL || j + 1 < n) o[ld] = (uint16_t)(w >> 16);
+      o += 2 * ld;
+    }
   } else {
-    // 4-byte stores on 4-byte boundaries: a row that starts between two takes
-    // its words one element further on, and its first element on its own
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-      if (r >= nr) break;
-      uint16_t *orow = reinterpret_cast<uint16_t *>(o + (long long)r * N);
-      const uint32_t a = stg[r * kPitchW + lane], b = stg[r * kPitchW + lane + 1];
-      const int odd = (int)(reinterpret_cast<uintptr_t>(orow) >> 1) & 1;
-      const int e = 2 * lane + odd;
-      if (e + 1 < n)
-        *reinterpret_cast<uint32_t *>(orow + e) = odd ? __byte_perm(a, b, 0x5432) : a;
-      else if (e < n)
-        orow[e] = (uint16_t)(odd ? a >> 16 : a);
-      if (odd && lane == 0) orow[0] = (uint16_t)a;
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) {
+      if (FULL || j < n) *g = f[j];
+      g += ld;
     }
   }
 }
 
-__device__ __forceinline__ float activate(float y, int act) {
-  if (act == TOCR_ACT_RELU) return y < 0.f ? 0.f : y;  // keeps NaN
-  if (act == TOCR_ACT_HARDSWISH) return y * (fminf(fmaxf(y + 3.f, 0.f), 6.f) * (1.f / 6.f));
-  return y;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
+// Tiles blockIdx.x, blockIdx.x + gridDim.x, ...: channels fastest, so that the
+// CTAs share few operand tiles at a time, and no division from tile to tile.
+struct TileWalk {
+  int ni, mi, dn, dm, tiles_n;
+  long long left;
+  __device__ __forceinline__ TileWalk(const LinParams &p) {
+    tiles_n = p.tiles_n;
+    ni = blockIdx.x % tiles_n;
+    mi = blockIdx.x / tiles_n;
+    dn = gridDim.x % tiles_n;
+    dm = gridDim.x / tiles_n;
+    left = (p.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;  // the grid has no idle CTA
+  }
+  __device__ __forceinline__ bool done() const { return left <= 0; }
+  __device__ __forceinline__ void next() {
+    --left;
+    ni += dn;
+    mi += dm;
+    if (ni >= tiles_n) {
+      ni -= tiles_n;
+      ++mi;
+    }
+  }
+};
 
 // SMALLK: |sum| < 2^22, so an s32 becomes fp32 by adding it to the bits of
 // 1.5 * 2^23 (two full-rate instructions; the conversion instruction runs at an
 // eighth of their rate and would bound layers of small K).
-template <typename T, int BN, bool SMALLK>
+template <typename T, bool SMALLK>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                  const LinParams p) {
-  using C = Cfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
-  uint64_t *empty = full + C::STAGES;
-  uint64_t *acc_full = empty + C::STAGES;  // [2]
-  uint64_t *acc_empty = acc_full + 2;      // [2]
-  uint32_t *s_tmem = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
-  volatile int *s_abort = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 4);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kOffBar);
+  uint64_t *empty = full + kMaxStages;
+  uint64_t *acc_full = empty + kMaxStages;  // [2]
+  uint64_t *acc_empty = acc_full + 2;       // [2]
+  uint32_t *s_tmem = reinterpret_cast<uint32_t *>(smem + kOffMisc);
+  volatile int *s_abort = reinterpret_cast<volatile int *>(smem + kOffMisc + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
+    for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -348,186 +342,201 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(s_tmem, C::TMEM);
+    tmem_alloc(s_tmem, 2 * kMaxBT);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  const int KS = p.ksteps;
+  const int KS = p.ksteps, stage = kStageA + p.bt * 128;
+  uint8_t *ring = smem + kOffRing;
 
   if (warp == 0) {
     if (elect_one()) {
       tma_prefetch_desc(&xmap);
       tma_prefetch_desc(&wmap);
-      long long j = 0;
+      int s = 0, used = 0;  // slot, slots ever filled
+      uint32_t phase = 0;
       bool ok = true;
-      for (long long t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
-        const int m0 = (int)(t / p.tiles_n) * kBM, n0 = (int)(t % p.tiles_n) * BN;
-        for (int k = 0; k < KS; ++k, ++j) {
-          const int s = (int)(j % C::STAGES);
-          const uint32_t u = (uint32_t)(j / C::STAGES);
-          if (u > 0 && !mbar_wait_bounded(&empty[s], (u - 1) & 1, s_abort, p.err, 81)) {
+      for (TileWalk t(p); ok && !t.done(); t.next()) {
+        const int m0 = t.mi * p.bt, n0 = t.ni * kBM;
+        for (int k = 0; k < KS; ++k) {
+          if (used == p.stages && !mbar_wait_bounded(&empty[s], phase ^ 1, s_abort, p.err, 81)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[s], C::STAGE);
-          tma_load_2d(smem + s * C::STAGE, &xmap, &full[s], 128 * k, m0);
-          tma_load_2d(smem + s * C::STAGE + C::STAGE_A, &wmap, &full[s], 128 * k, n0);
+          mbar_arrive_expect_tx(&full[s], stage);
+          tma_load_2d(ring + s * stage, &wmap, &full[s], 128 * k, n0);
+          tma_load_2d(ring + s * stage + kStageA, &xmap, &full[s], 128 * k, m0);
+          if (used < p.stages) ++used;
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
       }
       if (*s_abort) {  // leave no copy in flight
-        for (long long i = j > C::STAGES ? j - C::STAGES : 0; i < j; ++i) {
+        for (int i = 0; i < used; ++i) {
           const long long t0 = clock64();
-          while (!mbar_try_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1))
+          while (!mbar_try_wait(&full[i], i < s ? phase : phase ^ 1))
             if (clock64() - t0 > (1ll << 30)) break;
         }
       }
     }
   } else if (warp == 1) {
     if (elect_one()) {
-      constexpr uint32_t idesc = idesc_i8(kBM, BN);
-      long long j = 0;
-      int i = 0;
+      const uint32_t idesc = idesc_i8(kBM, p.bt);
+      const uint64_t desc0 = sw128_kmajor_desc(smem_u32(ring));
+      int s = 0;
+      uint32_t phase = 0;
+      Ring<2> acc;
       bool ok = true;
-      for (long long t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++i) {
-        const int b = i & 1;
-        if (i > 1 && !mbar_wait_bounded(&acc_empty[b], (uint32_t)((i >> 1) - 1) & 1, s_abort, p.err, 82))
+      for (TileWalk t(p); ok && !t.done(); t.next()) {
+        if (!acc.first && !mbar_wait_bounded(&acc_empty[acc.i], acc.phase ^ 1, s_abort, p.err, 82))
           break;
         tc_fence_after();
-        for (int k = 0; k < KS; ++k, ++j) {
-          const int s = (int)(j % C::STAGES);
-          if (!mbar_wait_bounded(&full[s], (uint32_t)(j / C::STAGES) & 1, s_abort, p.err, 83)) {
+        const uint32_t d = tmem + acc.i * kMaxBT;
+        for (int k = 0; k < KS; ++k) {
+          if (!mbar_wait_bounded(&full[s], phase, s_abort, p.err, 83)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + s * C::STAGE), w = a + C::STAGE_A;
+          const uint64_t a = desc0 + (uint64_t)((s * stage) >> 4);
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            mma_i8(tmem + (uint32_t)(b * BN), sw128_kmajor_desc(a + 32u * q),
-                   sw128_kmajor_desc(w + 32u * q), idesc, k > 0 || q > 0 ? 1u : 0u);
+            mma_i8(d, a + 2 * q, a + (kStageA >> 4) + 2 * q, idesc, k > 0 || q > 0 ? 1u : 0u);
           mma_commit(&empty[s]);
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
-        mma_commit(&acc_full[b]);
+        mma_commit(&acc_full[acc.i]);
+        acc.next();
       }
     }
   } else {
     const int ew = warp - kEpiWarp0;
-    const int half = ew >> 2;   // its columns of the tile
+    const int g = ew >> 2;      // takes units g, g + 4, ... of the tile's tokens
     const int quad = warp & 3;  // the TMEM lanes a warp may read
-    uint32_t *stg = reinterpret_cast<uint32_t *>(smem + C::OFF_STG) + ew * 32 * kPitchW;
-    float2 *cols = reinterpret_cast<float2 *>(smem + C::OFF_COL) + ew * 64;
-    constexpr int HC = BN / 2;                 // columns of a warp
-    constexpr int PC = 32 * (4 / sizeof(T)) < HC ? 32 * (4 / sizeof(T)) : HC;  // of a piece
-    constexpr int PER = 4 / sizeof(T);
+    const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16);
+    float *slice = reinterpret_cast<float *>(smem + kOffSx) + ew * 128;
     T *y = static_cast<T *>(p.y);
-    int i = 0;
-    for (long long t = blockIdx.x; t < p.tiles; t += gridDim.x, ++i) {
-      const int b = i & 1;
-      const long long row0 = t / p.tiles_n * kBM + quad * 32;
-      const int n0 = (int)(t % p.tiles_n) * BN + half * HC;
-      const float sx = row0 + lane < p.rows ? __ldg(p.sx + row0 + lane) : 0.f;
-      if (!mbar_wait_bounded(&acc_full[b], (uint32_t)(i >> 1) & 1, s_abort, p.err, 84)) break;
+    // a tile's channel scale and bias, and the scales of the warp's tokens,
+    // loaded while the tile before is worked on
+    float nsw = 0.f, nb = 0.f, ns0 = 0.f, ns1 = 0.f;
+    auto prefetch = [&](const TileWalk &t) {
+      const int n = t.ni * kBM + quad * 32 + lane;
+      const long long m =
+          (long long)t.mi * p.bt + (g + 4 * (lane / kUnit)) * kUnit + lane % kUnit;
+      nsw = n < p.N ? __ldg(p.sw + n) : 0.f;
+      nb = n < p.N && p.bias ? __ldg(p.bias + n) : 0.f;
+      ns0 = m < p.rows ? __ldg(p.sx + m) : 0.f;
+      ns1 = m + 8 * kUnit < p.rows ? __ldg(p.sx + m + 8 * kUnit) : 0.f;
+    };
+    TileWalk ahead(p);
+    if (!ahead.done()) prefetch(ahead);
+    Ring<2> acc;
+    for (TileWalk t(p); !t.done(); t.next(), acc.next()) {
+      const int n = t.ni * kBM + quad * 32 + lane;
+      const long long m0 = (long long)t.mi * p.bt;
+      const uint64_t sw2 = pk(nsw, nsw), b2 = pk(nb, nb);
+      float *sx = slice + acc.i * 64;
+      sx[lane] = ns0;
+      sx[32 + lane] = ns1;
+      __syncwarp();
+      ahead.next();
+      if (!ahead.done()) prefetch(ahead);
+      if (!mbar_wait_bounded(&acc_full[acc.i], acc.phase, s_abort, p.err, 84)) break;
       tc_fence_after();
-      const uint32_t ta = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * BN + half * HC);
-#pragma unroll 1
-      for (int c = 0; c < HC; c += PC) {
-        if (n0 + c >= p.N) break;
-        __syncwarp();
+      const uint32_t ta = tl + acc.i * kMaxBT;
+      const int units = p.bt / kUnit;
 #pragma unroll
-        for (int g = 0; g < PC; g += 32) {
-          const int n = n0 + c + g + lane;
-          cols[g + lane] = n < p.N ? make_float2(__ldg(p.sw + n), p.bias ? __ldg(p.bias + n) : 0.f)
-                                   : make_float2(0.f, 0.f);
-        }
-        __syncwarp();
+      for (int k = 0; k < kMaxBT / kUnit / 4; ++k) {
+        const int u = g + 4 * k;
+        if (u >= units) break;
+        uint32_t v[kUnit];
+        tmem_ld16(ta + u * kUnit, v);
+        tmem_ld_wait(v);
+        float f[kUnit];
+        const ulonglong2 *sq = reinterpret_cast<const ulonglong2 *>(sx + k * kUnit);
 #pragma unroll
-        for (int g = 0; g < PC; g += 32) {
-          uint32_t v[32];
-          tmem_ld32(ta + c + g, v);
-          tmem_ld_wait(v);
-          uint32_t o[32 / PER];
+        for (int j = 0; j < kUnit; j += 4) {
+          const ulonglong2 s4 = sq[j / 4];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float4 cc = *reinterpret_cast<const float4 *>(&cols[g + e]);
-            const float a0 = SMALLK ? __uint_as_float(v[e] + 0x4B400000u) - 12582912.f
-                                    : (float)(int)v[e];
-            const float a1 = SMALLK ? __uint_as_float(v[e + 1] + 0x4B400000u) - 12582912.f
-                                    : (float)(int)v[e + 1];
-            const float y0 = activate(fmaf(a0 * sx, cc.x, cc.y), p.act);
-            const float y1 = activate(fmaf(a1 * sx, cc.z, cc.w), p.act);
-            if constexpr (PER == 2) {
-              o[e / 2] = pack2<T>(y0, y1);
-            } else {
-              o[e] = __float_as_uint(y0);
-              o[e + 1] = __float_as_uint(y1);
-            }
+          for (int h = 0; h < 4; h += 2) {
+            uint64_t a;
+            if (SMALLK)
+              a = add2(pk(__uint_as_float(v[j + h] + 0x4B400000u),
+                          __uint_as_float(v[j + h + 1] + 0x4B400000u)),
+                       pk(-12582912.f, -12582912.f));
+            else
+              a = pk((float)(int)v[j + h], (float)(int)v[j + h + 1]);
+            upk(fma2(mul2(a, h ? s4.y : s4.x), sw2, b2), f[j + h], f[j + h + 1]);
           }
-          uint4 *so = reinterpret_cast<uint4 *>(stg + lane * kPitchW + g / PER);
-#pragma unroll
-          for (int e = 0; e < 8 / PER; ++e)
-            so[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
-        __syncwarp();
-        if (row0 < p.rows) write_piece<T, PC>(y, row0, p.rows, p.N, n0 + c, p.vec, stg, lane);
+        if (p.act) {
+#pragma unroll
+          for (int j = 0; j < kUnit; ++j) f[j] = activate(f[j], p.act);
+        }
+        const long long m = m0 + u * kUnit;
+        if (n < p.N && m < p.rows) {
+          T *o = y + m * p.N + n;
+          if (m + kUnit <= p.rows)
+            store_unit<T, true>(o, p.N, f, kUnit);
+          else
+            store_unit<T, false>(o, p.N, f, (int)(p.rows - m));
+        }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[b]);
+      if (lane == 0) mbar_arrive(&acc_empty[acc.i]);
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::TMEM);
+    tmem_dealloc(tmem, 2 * kMaxBT);
   }
 }
 
-template <typename T, int BN, bool SMALLK>
-int launch_product(const void *xq, const void *wq, const LinParams &p, int pitch, cudaStream_t st) {
-  using C = Cfg<BN>;
+template <typename T, bool SMALLK>
+int launch_product(const void *xq, const void *wq, LinParams p, int pitch, cudaStream_t st) {
   CUtensorMap xm, wm;
-  int rc = tma_map_rows(&xm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, pitch, p.rows, pitch, kBM);
+  int rc = tma_map_rows(&xm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, pitch, p.rows, pitch, p.bt);
   if (rc) return rc;
-  rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, pitch, p.N, pitch, BN);
+  rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, pitch, p.N, pitch, kBM);
   if (rc) return rc;
-  cudaError_t e = cudaFuncSetAttribute(linear_i8_kernel<T, BN, SMALLK>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  p.stages = kRingBytes / (kStageA + p.bt * 128);
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  auto *kernel = linear_i8_kernel<T, SMALLK>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return set_error(TOCR_ERR_CUDA, "tocr_linear_i8: %s", cudaGetErrorString(e));
   const int grid = (int)(p.tiles < sm_count() ? p.tiles : sm_count());
-  linear_i8_kernel<T, BN, SMALLK><<<grid, kThreads, C::SMEM, st>>>(xm, wm, p);
+  kernel<<<grid, kThreads, kSmem, st>>>(xm, wm, p);
   return check_launch("linear_i8_kernel");
 }
 
-template <typename T, int BN>
-int product_bn(const void *xq, const void *wq, LinParams p, int pitch, cudaStream_t st) {
-  p.tiles_n = (p.N + BN - 1) / BN;
-  p.tiles = (p.rows + kBM - 1) / kBM * p.tiles_n;
-  // 127^2 K < 2^22
-  return p.K <= 260 ? launch_product<T, BN, true>(xq, wq, p, pitch, st)
-                    : launch_product<T, BN, false>(xq, wq, p, pitch, st);
-}
-
 template <typename T>
-int product(const void *xq, const void *wq, const LinParams &p, int pitch, cudaStream_t st) {
-  // the tile width whose waves of CTAs take least: a tile costs its columns and
-  // a fixed part worth about 64 columns
-  const long long tm = (p.rows + kBM - 1) / kBM, sms = sm_count();
+int product(const void *xq, const void *wq, LinParams p, int K, int pitch, cudaStream_t st) {
+  p.tiles_n = (p.N + kBM - 1) / kBM;
+  // the tokens of a tile for which the waves of CTAs take least: a tile costs
+  // its tokens and a fixed part worth about 64 tokens
+  const long long sms = sm_count();
   long long best = -1;
-  int bn = 256;
-  for (int b = 256; b >= 64; b /= 2) {
-    const long long cost = (tm * ((p.N + b - 1) / b) + sms - 1) / sms * (b + 64);
+  for (int bt = kMaxBT; bt >= kUnit; bt -= kUnit) {
+    const long long cost = ((long long)p.tiles_n * ((p.rows + bt - 1) / bt) + sms - 1) / sms * (bt + 64);
     if (best < 0 || cost < best) {
       best = cost;
-      bn = b;
+      p.bt = bt;
     }
   }
-  if (bn == 256) return product_bn<T, 256>(xq, wq, p, pitch, st);
-  if (bn == 128) return product_bn<T, 128>(xq, wq, p, pitch, st);
-  return product_bn<T, 64>(xq, wq, p, pitch, st);
+  p.tiles = p.tiles_n * ((p.rows + p.bt - 1) / p.bt);
+  return K <= 260 ? launch_product<T, true>(xq, wq, p, pitch, st)  // 127^2 K < 2^22
+                  : launch_product<T, false>(xq, wq, p, pitch, st);
 }
 
 constexpr long long kMaxRows = 1ll << 24;
@@ -557,15 +566,13 @@ int run_product(const void *xq, const float *sx, long long rows, int K, const vo
   p.y = y;
   p.rows = rows;
   p.N = N;
-  p.K = K;
   p.ksteps = (K + 127) / 128;
   p.act = act;
-  p.vec = aligned(y, 16) && (size_t)N * (out_dtype == TOCR_DTYPE_F32 ? 4 : 2) % 16 == 0;
   p.err = err;
   const int pitch = (K + 15) / 16 * 16;
-  if (out_dtype == TOCR_DTYPE_F16) return product<__half>(xq, wq, p, pitch, st);
-  if (out_dtype == TOCR_DTYPE_BF16) return product<__nv_bfloat16>(xq, wq, p, pitch, st);
-  return product<float>(xq, wq, p, pitch, st);
+  if (out_dtype == TOCR_DTYPE_F16) return product<__half>(xq, wq, p, K, pitch, st);
+  if (out_dtype == TOCR_DTYPE_BF16) return product<__nv_bfloat16>(xq, wq, p, K, pitch, st);
+  return product<float>(xq, wq, p, K, pitch, st);
 }
 
 size_t codes_bytes(long long rows, int K) {
@@ -587,6 +594,8 @@ TOCR_API int tocr_quant_rows_i8(const void *d_x, int x_dtype, long long rows, in
   TOCR_REQUIRE(is_dtype(x_dtype), "tocr_quant_rows_i8: unknown type %d", x_dtype);
   if (rows == 0) return TOCR_OK;
   TOCR_REQUIRE(d_x && d_codes && d_scales, "tocr_quant_rows_i8: null pointer");
+  TOCR_REQUIRE(aligned(d_x, x_dtype == TOCR_DTYPE_F32 ? 4 : 2),
+               "tocr_quant_rows_i8: x must be aligned to its element");
   TOCR_REQUIRE(aligned(d_codes, 16), "tocr_quant_rows_i8: the codes must be 16-byte aligned");
   return quant_rows(d_x, x_dtype, rows, K, static_cast<int8_t *>(d_codes), d_scales,
                     as_stream(stream));
@@ -601,6 +610,8 @@ TOCR_API int tocr_linear_i8_codes(const void *d_xq, const float *d_sx, long long
   TOCR_REQUIRE(d_xq && d_sx && d_wq && d_sw && d_y && d_err, "tocr_linear_i8_codes: null pointer");
   TOCR_REQUIRE(aligned(d_xq, 16) && aligned(d_wq, 16),
                "tocr_linear_i8_codes: the codes must be 16-byte aligned");
+  TOCR_REQUIRE(aligned(d_y, out_dtype == TOCR_DTYPE_F32 ? 4 : 2),
+               "tocr_linear_i8_codes: y must be aligned to its element");
   return run_product(d_xq, d_sx, rows, K, d_wq, d_sw, d_bias, N, act, out_dtype, d_y, d_err,
                      as_stream(stream));
 }
@@ -621,6 +632,9 @@ TOCR_API int tocr_linear_i8(const void *d_x, int x_dtype, long long rows, int K,
   if (rows == 0) return TOCR_OK;
   TOCR_REQUIRE(d_x && d_wq && d_sw && d_y && d_workspace && d_err, "tocr_linear_i8: null pointer");
   TOCR_REQUIRE(aligned(d_wq, 16), "tocr_linear_i8: the codes must be 16-byte aligned");
+  TOCR_REQUIRE(aligned(d_x, x_dtype == TOCR_DTYPE_F32 ? 4 : 2) &&
+                   aligned(d_y, out_dtype == TOCR_DTYPE_F32 ? 4 : 2),
+               "tocr_linear_i8: x and y must be aligned to their elements");
   TOCR_REQUIRE(aligned(d_workspace, 256) && workspace_bytes >= codes_bytes(rows, K) + (size_t)rows * 4,
                "tocr_linear_i8: the workspace must be 256-byte aligned and hold %zu bytes",
                codes_bytes(rows, K) + (size_t)rows * 4);
