@@ -48,6 +48,27 @@ int sm_count() {
   return cached_sms;
 }
 
+int allow_dynamic_smem(const void *kernel, int bytes, const char *what) {
+  // (kernel, device) pairs that this thread has raised lately, newest last
+  struct Pair {
+    const void *kernel;
+    int dev;
+  };
+  constexpr int kPairs = 64;
+  static thread_local Pair raised[kPairs] = {};
+  static thread_local unsigned next = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) {
+    for (const Pair &p : raised)
+      if (p.kernel == kernel && p.dev == dev) return TOCR_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  }
+  if (e != cudaSuccess) return set_error(TOCR_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  raised[next++ % kPairs] = {kernel, dev};
+  return TOCR_OK;
+}
+
 }  // namespace tocr
 
 extern "C" {

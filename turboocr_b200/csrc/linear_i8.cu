@@ -126,6 +126,7 @@ quant_rows_kernel(const T *__restrict__ x, long long rows, int K, int pitch,
   constexpr int E = 16 / sizeof(T);
   constexpr int TEAMS = kQuantThreads / TEAM;
   __shared__ uint32_t smax[kQuantThreads / 32];
+  release_next();
   const int tid = threadIdx.x % TEAM;
   const long long row = (long long)blockIdx.x * TEAMS + threadIdx.x / TEAM;
   const bool live = row < rows;
@@ -247,6 +248,7 @@ struct LinParams {
   int tiles_n;
   long long tiles;
   int act;
+  bool behind_quant;             // launched behind the quantiser of the same call
   int *err;
 };
 
@@ -349,6 +351,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  after_previous();
   const int KS = p.ksteps, stage = kStageA + p.bt * 128;
   uint8_t *ring = smem + kOffRing;
 
@@ -513,9 +516,11 @@ int launch_product(const void *xq, const void *wq, LinParams p, int pitch, cudaS
   p.stages = kRingBytes / (kStageA + p.bt * 128);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   auto *kernel = linear_i8_kernel<T, SMALLK>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (e != cudaSuccess) return set_error(TOCR_ERR_CUDA, "tocr_linear_i8: %s", cudaGetErrorString(e));
+  rc = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), kSmem, "linear_i8_kernel");
+  if (rc) return rc;
   const int grid = (int)(p.tiles < sm_count() ? p.tiles : sm_count());
+  if (p.behind_quant)
+    return launch_overlapped("linear_i8_kernel", kernel, grid, kThreads, kSmem, st, xm, wm, p);
   kernel<<<grid, kThreads, kSmem, st>>>(xm, wm, p);
   return check_launch("linear_i8_kernel");
 }
@@ -558,8 +563,9 @@ int check_linear(const char *fn, long long rows, int K, int N, int act, int out_
 
 int run_product(const void *xq, const float *sx, long long rows, int K, const void *wq,
                 const float *sw, const float *bias, int N, int act, int out_dtype, void *y,
-                int *err, cudaStream_t st) {
+                int *err, bool behind_quant, cudaStream_t st) {
   LinParams p{};
+  p.behind_quant = behind_quant;
   p.sx = sx;
   p.sw = sw;
   p.bias = bias;
@@ -613,7 +619,7 @@ TOCR_API int tocr_linear_i8_codes(const void *d_xq, const float *d_sx, long long
   TOCR_REQUIRE(aligned(d_y, out_dtype == TOCR_DTYPE_F32 ? 4 : 2),
                "tocr_linear_i8_codes: y must be aligned to its element");
   return run_product(d_xq, d_sx, rows, K, d_wq, d_sw, d_bias, N, act, out_dtype, d_y, d_err,
-                     as_stream(stream));
+                     false, as_stream(stream));
 }
 
 TOCR_API size_t tocr_linear_i8_workspace_bytes(long long rows, int K) {
@@ -643,7 +649,8 @@ TOCR_API int tocr_linear_i8(const void *d_x, int x_dtype, long long rows, int K,
   float *sx = reinterpret_cast<float *>(q + codes_bytes(rows, K));
   rc = quant_rows(d_x, x_dtype, rows, K, q, sx, st);
   if (rc) return rc;
-  return run_product(q, sx, rows, K, d_wq, d_sw, d_bias, N, act, out_dtype, d_y, d_err, st);
+  return run_product(q, sx, rows, K, d_wq, d_sw, d_bias, N, act, out_dtype, d_y, d_err,
+                     true, st);
 }
 
 }  // extern "C"

@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kRowBlock)
 ce_count_kernel(const void *targets, bool wide, int rows, int V, const float *g, int *cnt,
                 float *gblk) {
   __shared__ float sm[kRowBlock / 32];
+  release_next();
   const long long i = (long long)blockIdx.x * kRowBlock + threadIdx.x;
   const bool keep = i < rows && target_of(targets, wide, i, V) >= 0;
   const int n = __syncthreads_count(keep);
@@ -194,6 +195,8 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
   __shared__ float s_gmax;
   __shared__ int s_dst[kRowBlock];  // place of each row of the block, -1: padding
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  release_next();
+  if (!p.direct) after_previous();
   // kept rows before this block, and the largest weight of all
   int before = 0;
   float gm = 0.f;
@@ -316,12 +319,8 @@ struct Cuts {
   }
   // first step of range c
   __device__ long long at(int c) const { return c >= G ? total : q * c + r * c / G; }
-  // the range that holds step `it`
-  __device__ int owner(long long it) const {
-    int c = (int)(it / (q + 1));
-    while (c + 1 < G && at(c + 1) <= it) ++c;
-    return c;
-  }
+  // the range that holds step `it`: at(c) = floor(total c / G) <= it
+  __device__ int owner(long long it) const { return (int)(((it + 1) * G - 1) / total); }
 };
 
 // ------------------------------------------------------------ small parts ---
@@ -505,6 +504,7 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  after_previous();
   const int n = p.hdr->n;
   const int NC = p.chunks;
   const long long total = (long long)((n + kTile - 1) / kTile) * NC;
@@ -698,6 +698,7 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
       it += cnt;
     }
   }
+  release_next();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -743,6 +744,7 @@ ce_loss_kernel(const FwdParams p, const uint8_t *w, const float *bias, const int
   __shared__ int s_first, s_last;
   __shared__ float2 s_run[8][32];
   __shared__ float s_lt[32];
+  after_previous();
   const int n = p.hdr->n;
   const int tile = blockIdx.x / (kTile / 32), r0 = blockIdx.x % (kTile / 32) * 32;
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
@@ -892,6 +894,7 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  after_previous();
   const BwdLine line(p.hdr, C::CN, p.chunks_v, p.want_x, p.tiles_w);
   const Cuts cuts(line.total, gridDim.x);
   const long long it0 = cuts.at(blockIdx.x), it1 = cuts.at(blockIdx.x + 1);
@@ -1156,6 +1159,7 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
       it += cnt;
     }
   }
+  release_next();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -1171,6 +1175,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(256)
 ce_join_kernel(const BwdParams p, int cn, int KP, int grid) {
   __shared__ int s_tile, s_dw, s_last;
+  after_previous();
   if (threadIdx.x == 0) {
     s_tile = -1;
     const BwdLine line(p.hdr, cn, p.chunks_v, p.want_x, p.tiles_w);
@@ -1230,13 +1235,6 @@ ce_join_kernel(const BwdParams p, int cn, int KP, int grid) {
 }
 
 // ----------------------------------------------------------------- host -----
-template <typename F>
-int allow_smem(F *kernel, int bytes, const char *what) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == cudaSuccess ? TOCR_OK
-                          : set_error(TOCR_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
 int grid_for(long long steps, int least) {
   const long long g = (steps + least - 1) / least;
   const int most = sm_count() < kMaxGrid ? sm_count() : kMaxGrid;
@@ -1250,10 +1248,11 @@ int launch_fwd(const FwdParams &p, const void *w, int grid, cudaStream_t st) {
   int rc = tma_map_rows(&wm, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                         2, w, p.K, p.V, 2ll * p.K, C::CN);
   if (rc) return rc;
-  rc = allow_smem(ce_fwd_kernel<KA, BF16>, C::SMEM, "tocr_rec_head_ce");
+  rc = allow_dynamic_smem(reinterpret_cast<const void *>(ce_fwd_kernel<KA, BF16>), C::SMEM,
+                          "ce_fwd_kernel");
   if (rc) return rc;
-  ce_fwd_kernel<KA, BF16><<<grid, kThreads, C::SMEM, st>>>(wm, p);
-  return check_launch("ce_fwd_kernel");
+  return launch_overlapped("ce_fwd_kernel", ce_fwd_kernel<KA, BF16>, grid, kThreads, C::SMEM, st, wm,
+                           p);
 }
 
 template <int KA, bool BF16>
@@ -1266,13 +1265,14 @@ int launch_bwd(const BwdParams &p, int rows_pad, int grid, cudaStream_t st) {
   if (rc) return rc;
   rc = tma_map_rows(&xm, ty, 2, p.xc, p.K, rows_pad, 2ll * p.K, C::CN);
   if (rc) return rc;
-  rc = allow_smem(ce_bwd_kernel<KA, BF16>, C::SMEM, "tocr_rec_head_ce_backward");
+  rc = allow_dynamic_smem(reinterpret_cast<const void *>(ce_bwd_kernel<KA, BF16>), C::SMEM,
+                          "ce_bwd_kernel");
   if (rc) return rc;
-  ce_bwd_kernel<KA, BF16><<<grid, kThreads, C::SMEM, st>>>(wm, xm, p);
-  rc = check_launch("ce_bwd_kernel");
+  rc = launch_overlapped("ce_bwd_kernel", ce_bwd_kernel<KA, BF16>, grid, kThreads, C::SMEM, st, wm,
+                         xm, p);
   if (rc || grid == 1) return rc;
-  ce_join_kernel<BF16><<<dim3(grid - 1, 8), 256, 0, st>>>(p, C::CN, C::KP, grid);
-  return check_launch("ce_join_kernel");
+  return launch_overlapped("ce_join_kernel", ce_join_kernel<BF16>, dim3(grid - 1, 8), 256, 0, st, p,
+                           C::CN, C::KP, grid);
 }
 
 template <bool BWD>
@@ -1311,6 +1311,9 @@ int launch_place(const Workspace &ws, const void *targets, bool wide, int rows, 
   p.nlse = ws.nlse;
   p.gc = ws.gc;
   p.gs = ws.gs;
+  if (!direct)
+    return launch_overlapped("ce_place_kernel", ce_place_kernel<BWD>, dim3(blocks, 8), kRowBlock, 0,
+                             st, p);
   ce_place_kernel<BWD><<<dim3(blocks, 8), kRowBlock, 0, st>>>(p);
   return check_launch("ce_place_kernel");
 }
@@ -1379,9 +1382,9 @@ TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *
     default: rc = bf ? launch_fwd<4, true>(p, d_w, grid, st) : launch_fwd<4, false>(p, d_w, grid, st);
   }
   if (rc) return rc;
-  (bf ? ce_loss_kernel<true> : ce_loss_kernel<false>)<<<tiles * (kTile / 32), 256, 0, st>>>(
-      p, static_cast<const uint8_t *>(d_w), d_bias, ws.tgt, grid, d_loss, d_lse);
-  return check_launch("ce_loss_kernel");
+  return launch_overlapped("ce_loss_kernel", bf ? ce_loss_kernel<true> : ce_loss_kernel<false>,
+                           tiles * (kTile / 32), 256, 0, st, p, static_cast<const uint8_t *>(d_w),
+                           d_bias, ws.tgt, grid, d_loss, d_lse);
 }
 
 TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, const float *d_bias,

@@ -36,6 +36,41 @@ inline bool aligned(const void *p, size_t a) {
 // SM count of the current device, cached per device.
 int sm_count();
 
+// Launches a kernel that may begin while the kernel before it in the stream
+// still runs, and that waits for it itself (after_previous()) before it touches
+// memory: its set-up overlaps the other's end. For kernels inside one call only,
+// behind a first one that is launched as usual.
+template <typename... P, typename... A>
+int launch_overlapped(const char *what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
+                      cudaStream_t st, A &&...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e == cudaSuccess ? TOCR_OK
+                          : set_error(TOCR_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// lets the next kernel's set-up begin once every block of this one got here
+__device__ __forceinline__ void release_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+#endif
+
+// Allows `kernel` `bytes` of dynamic shared memory on the current device (asked
+// of the driver once per kernel and device).
+int allow_dynamic_smem(const void *kernel, int bytes, const char *what);
+
 }  // namespace tocr
 
 // Common prologue for a compute entry: clear error, honour injection.

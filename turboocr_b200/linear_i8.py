@@ -19,6 +19,9 @@ from ._lib import call, lib
 
 ACTS = {"none": 0, "relu": 1, "hardswish": 2}  # TOCR_ACT_*
 _FLOATS = tuple(DTYPES)
+_F32 = (torch.float32,)
+_I32 = (torch.int32,)
+_I8 = (torch.int8,)
 
 
 def pitch(K: int) -> int:
@@ -33,13 +36,13 @@ def quantize_rows(x: torch.Tensor, *, stream=None) -> tuple[torch.Tensor, torch.
     NaN gets the scale NaN and codes 0."""
     if x.dim() != 2:
         raise ValueError("x is [rows, K]")
-    dev = x.device
-    px = dense(x, "x", dev, *_FLOATS)
+    dev = x.get_device()
+    px = dense(x, "x", dev, _FLOATS)
     rows, K = x.shape
 
     def launch(s):
-        codes = torch.empty(rows, pitch(K), dtype=torch.int8, device=dev)
-        scales = torch.empty(rows, dtype=torch.float32, device=dev)
+        codes = torch.empty(rows, pitch(K), dtype=torch.int8, device=x.device)
+        scales = torch.empty(rows, dtype=torch.float32, device=x.device)
         call("tocr_quant_rows_i8", px, DTYPES[x.dtype], rows, K, codes.data_ptr(),
              scales.data_ptr(), s)
         return codes, scales
@@ -49,21 +52,21 @@ def quantize_rows(x: torch.Tensor, *, stream=None) -> tuple[torch.Tensor, torch.
 
 def _weights(wq, ws, bias, K, dev, act, out_dtype, err):
     N = wq.shape[0]
-    shaped(wq, "wq", N, pitch(K))
-    shaped(ws, "ws", N)
+    shaped(wq, "wq", (N, pitch(K)))
+    shaped(ws, "ws", (N,))
     pb = None
     if bias is not None:
-        shaped(bias, "bias", N)
-        pb = dense(bias, "bias", dev, torch.float32)
+        shaped(bias, "bias", (N,))
+        pb = dense(bias, "bias", dev, _F32)
     if act not in ACTS:
         raise ValueError(f"act must be one of {', '.join(ACTS)}, not {act!r}")
     if out_dtype not in DTYPES:
         raise ValueError(f"out_dtype must be one of {', '.join(map(str, DTYPES))}")
-    pe = dense(err, "err", dev, torch.int32)
-    if err.numel() < 1:
+    pe = dense(err, "err", dev, _I32)
+    if not err.numel():
         raise ValueError("err must hold one int32")
-    return N, pe, (dense(wq, "wq", dev, torch.int8), dense(ws, "ws", dev, torch.float32), pb, N,
-                   ACTS[act], DTYPES[out_dtype])
+    return N, pe, (dense(wq, "wq", dev, _I8), dense(ws, "ws", dev, _F32), pb, N, ACTS[act],
+                   DTYPES[out_dtype])
 
 
 def linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias: torch.Tensor | None = None,
@@ -74,16 +77,16 @@ def linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias: torch.Tens
     out_dtype: x's by default. The sum is exact, the rest fp32, rounded once."""
     if x.dim() != 2 or wq.dim() != 2:
         raise ValueError("x is [rows, K], wq is [N, pitch(K)]")
-    dev = x.device
+    dev = x.get_device()
     rows, K = x.shape
-    px = dense(x, "x", dev, *_FLOATS)
+    px = dense(x, "x", dev, _FLOATS)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     N, pe, w = _weights(wq, ws, bias, K, dev, act, out_dtype, err)
 
     def launch(s):
-        y = torch.empty(rows, N, dtype=out_dtype, device=dev)
+        y = torch.empty(rows, N, dtype=out_dtype, device=x.device)
         n = lib().tocr_linear_i8_workspace_bytes(rows, K)
-        buf = torch.empty(n, dtype=torch.uint8, device=dev)
+        buf = torch.empty(n, dtype=torch.uint8, device=x.device)
         call("tocr_linear_i8", px, DTYPES[x.dtype], rows, K, *w, y.data_ptr(), buf.data_ptr(), n,
              pe, s)
         return y
@@ -98,15 +101,15 @@ def linear_codes(xq: torch.Tensor, sx: torch.Tensor, K: int, wq: torch.Tensor, w
     on the same activations quantise them once)."""
     if xq.dim() != 2 or wq.dim() != 2:
         raise ValueError("xq is [rows, pitch(K)], wq is [N, pitch(K)]")
-    dev = xq.device
+    dev = xq.get_device()
     rows = xq.shape[0]
-    shaped(xq, "xq", rows, pitch(K))
-    shaped(sx, "sx", rows)
-    px, psx = dense(xq, "xq", dev, torch.int8), dense(sx, "sx", dev, torch.float32)
+    shaped(xq, "xq", (rows, pitch(K)))
+    shaped(sx, "sx", (rows,))
+    px, psx = dense(xq, "xq", dev, _I8), dense(sx, "sx", dev, _F32)
     N, pe, w = _weights(wq, ws, bias, K, dev, act, out_dtype, err)
 
     def launch(s):
-        y = torch.empty(rows, N, dtype=out_dtype, device=dev)
+        y = torch.empty(rows, N, dtype=out_dtype, device=xq.device)
         call("tocr_linear_i8_codes", px, psx, rows, K, *w, y.data_ptr(), pe, s)
         return y
 

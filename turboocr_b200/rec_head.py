@@ -16,34 +16,33 @@ import torch
 from ._launch import DTYPES, dense, on, shaped
 from ._lib import call, lib
 
-_F32 = torch.float32
+_F32 = (torch.float32,)
+_I32 = (torch.int32,)
+_INTS = (torch.int32, torch.int64)
+_HALVES = (torch.float16, torch.bfloat16)
 
 
 def _common(feat, weight, bias, targets, err):
     if feat.dim() != 2 or weight.dim() != 2:
         raise ValueError("features are [rows, K], weights [classes, K]")
-    dev = feat.device
+    dev = feat.get_device()
     rows, K = feat.shape
     V = weight.shape[0]
-    shaped(weight, "weight", V, K)
-    shaped(targets, "targets", rows)
-    pf = dense(feat, "feat", dev, torch.float16, torch.bfloat16)
-    pw = dense(weight, "weight", dev, feat.dtype)
+    shaped(weight, "weight", (V, K))
+    shaped(targets, "targets", (rows,))
+    dt = feat.dtype
+    pf = dense(feat, "feat", dev, _HALVES)
+    pw = dense(weight, "weight", dev, (dt,))
     pb = None
     if bias is not None:
-        shaped(bias, "bias", V)
+        shaped(bias, "bias", (V,))
         pb = dense(bias, "bias", dev, _F32)
-    pt = dense(targets, "targets", dev, torch.int32, torch.int64)
-    pe = dense(err, "err", dev, torch.int32)
-    if err.numel() < 1:
+    pt = dense(targets, "targets", dev, _INTS)
+    pe = dense(err, "err", dev, _I32)
+    if not err.numel():
         raise ValueError("err must hold one int32")
     return (dev, rows, K, V, pe,
-            (pf, pw, pb, pt, int(targets.dtype == torch.int64), rows, K, V, DTYPES[feat.dtype]))
-
-
-def _workspace(rows, K, V, backward, dev):
-    n = lib().tocr_rec_head_ce_workspace_bytes(rows, K, V, backward)
-    return torch.empty(n, dtype=torch.uint8, device=dev), n
+            (pf, pw, pb, pt, targets.dtype is torch.int64, rows, K, V, DTYPES[dt]))
 
 
 def cross_entropy(feat: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
@@ -56,9 +55,10 @@ def cross_entropy(feat: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
     dev, rows, K, V, pe, args = _common(feat, weight, bias, targets, err)
 
     def launch(s):
-        loss = torch.empty(rows, dtype=_F32, device=dev)
-        lse = torch.empty(rows, dtype=_F32, device=dev)
-        ws, n = _workspace(rows, K, V, 0, dev)
+        loss = torch.empty(rows, dtype=torch.float32, device=feat.device)
+        lse = torch.empty_like(loss)
+        n = lib().tocr_rec_head_ce_workspace_bytes(rows, K, V, 0)
+        ws = torch.empty(n, dtype=torch.uint8, device=feat.device)
         call("tocr_rec_head_ce", *args, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), n, pe, s)
         return loss, lse
 
@@ -74,18 +74,20 @@ def cross_entropy_backward(feat: torch.Tensor, weight: torch.Tensor, bias: torch
     dfeat and dweight have the inputs' type, dbias is fp32 (None without a
     bias); a gradient that is not needed is None. Padding rows get zeros."""
     dev, rows, K, V, pe, args = _common(feat, weight, bias, targets, err)
-    shaped(lse, "lse", rows)
-    shaped(grad_loss, "grad_loss", rows)
+    shaped(lse, "lse", (rows,))
+    shaped(grad_loss, "grad_loss", (rows,))
     pl, pg = dense(lse, "lse", dev, _F32), dense(grad_loss, "grad_loss", dev, _F32)
 
     def launch(s):
         dfeat = torch.empty_like(feat) if need_feat else None
         dweight = torch.empty_like(weight) if need_weight else None
         dbias = torch.empty_like(bias) if need_bias and bias is not None else None
-        ws, n = _workspace(rows, K, V, 1, dev)
+        n = lib().tocr_rec_head_ce_workspace_bytes(rows, K, V, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=feat.device)
         call("tocr_rec_head_ce_backward", *args, pl, pg,
-             *[t.data_ptr() if t is not None else None for t in (dfeat, dweight, dbias)],
-             ws.data_ptr(), n, pe, s)
+             dfeat.data_ptr() if need_feat else None,
+             dweight.data_ptr() if need_weight else None,
+             dbias.data_ptr() if dbias is not None else None, ws.data_ptr(), n, pe, s)
         return dfeat, dweight, dbias
 
     return on(dev, stream, launch)
