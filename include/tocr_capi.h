@@ -191,9 +191,10 @@ TOCR_API int tocr_linear_i8_codes(const void *d_xq, const float *d_sx, long long
                                   const void *d_wq, const float *d_sw, const float *d_bias, int N,
                                   int act, int out_dtype, void *d_y, int *d_err, void *stream);
 
-/* The layer on activations as they are: tocr_quant_rows_i8 of d_x into the
- * workspace (256-byte aligned, tocr_linear_i8_workspace_bytes, scratch of one
- * call), then tocr_linear_i8_codes. */
+/* The layer on activations as they are: the same codes as tocr_quant_rows_i8
+ * makes of d_x, then as tocr_linear_i8_codes. The workspace (256-byte aligned,
+ * tocr_linear_i8_workspace_bytes) is scratch of one call, so calls that may
+ * overlap need their own; few tokens need none (0 bytes, NULL). */
 TOCR_API size_t tocr_linear_i8_workspace_bytes(long long rows, int K);
 TOCR_API int tocr_linear_i8(const void *d_x, int x_dtype, long long rows, int K, const void *d_wq,
                             const float *d_sw, const float *d_bias, int N, int act, int out_dtype,

@@ -32,7 +32,8 @@ COMMON = ["-O3", "-lineinfo", "-std=c++20", "-Xcompiler", "-fPIC", "-Xcompiler",
 LIBS = {
     "libtocr_b200.so": ["capi_common.cu", "ctc.cu", "preprocess.cu", "threshold.cu", "dwpw.cu",
                         "db.cu", "pagekernels.cu", "crop.cu", "jfa.cu", "cls.cu", "rec_head.cu", "dbhead.cu",
-                        "png.cu", "rec_ce.cu", "linear_i8.cu"],
+                        "png.cu", "rec_ce.cu", "linear_i8.cu",
+                        "linear_i8_rows.cu"],
     "libtocr_synth.so": ["synth.cu"],
 }
 # C++ host sources (reference-signature shims), built into libtocr_b200.so.

@@ -19,28 +19,21 @@
 // the epilogue keeps its channel's scale and bias in registers, and a warp
 // stores 32 neighbouring channels of one token with one instruction straight
 // from registers, whatever the alignment of y's rows (the dictionary's 18385
-// columns leave most of them off every boundary). One persistent CTA per SM:
+// columns leave most of them off every boundary; large outputs of that kind have
+// their own kernel, linear_i8_rows.cu). One persistent CTA per SM:
 // warp 0 loads 128 x 128-byte tiles of the weight codes and BT x 128-byte tiles
 // of the token codes by TMA (128-byte swizzle) into a ring, one thread of warp 1
 // issues tcgen05.mma kind::i8 into one of two TMEM accumulators, and sixteen
 // warps run the epilogue of the other.
-#include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
 #include <cmath>
-#include <cstdint>
-#include <type_traits>
 
-#include "tc_ptx.cuh"
-#include "tma_map.cuh"
-#include "tocr_common.cuh"
+#include "linear_i8.cuh"
 
 namespace tocr {
 namespace {
 
 using namespace ptx;
+using namespace linear;
 
 // --------------------------------------------------------------- quantiser --
 template <typename T>
@@ -239,34 +232,6 @@ constexpr int kOffRing = (kOffMisc + 16 + 1023) / 1024 * 1024;
 constexpr int kSmem = 226 * 1024;
 constexpr int kRingBytes = kSmem - 1024 - kOffRing;
 
-struct LinParams {
-  const float *sx, *sw, *bias;
-  void *y;
-  long long rows;
-  int N, ksteps;
-  int bt, stages;                // tokens of a tile, slots of the ring
-  int tiles_n;
-  long long tiles;
-  int act;
-  bool behind_quant;             // launched behind the quantiser of the same call
-  int *err;
-};
-
-__device__ __forceinline__ float activate(float y, int act) {
-  if (act == TOCR_ACT_RELU) return y < 0.f ? 0.f : y;  // keeps NaN
-  return y * (fminf(fmaxf(y + 3.f, 0.f), 6.f) * (1.f / 6.f));
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  if constexpr (std::is_same_v<T, __half>)
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // f[j] to token j's row: g, g + ld, ... for the first n of 16 tokens
 template <typename T, bool FULL>
 __device__ __forceinline__ void store_unit(T *g, long long ld, const float (&f)[kUnit], int n) {
@@ -288,34 +253,6 @@ __device__ __forceinline__ void store_unit(T *g, long long ld, const float (&f)[
   }
 }
 
-// Tiles blockIdx.x, blockIdx.x + gridDim.x, ...: channels fastest, so that the
-// CTAs share few operand tiles at a time, and no division from tile to tile.
-struct TileWalk {
-  int ni, mi, dn, dm, tiles_n;
-  long long left;
-  __device__ __forceinline__ TileWalk(const LinParams &p) {
-    tiles_n = p.tiles_n;
-    ni = blockIdx.x % tiles_n;
-    mi = blockIdx.x / tiles_n;
-    dn = gridDim.x % tiles_n;
-    dm = gridDim.x / tiles_n;
-    left = (p.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;  // the grid has no idle CTA
-  }
-  __device__ __forceinline__ bool done() const { return left <= 0; }
-  __device__ __forceinline__ void next() {
-    --left;
-    ni += dn;
-    mi += dm;
-    if (ni >= tiles_n) {
-      ni -= tiles_n;
-      ++mi;
-    }
-  }
-};
-
-// SMALLK: |sum| < 2^22, so an s32 becomes fp32 by adding it to the bits of
-// 1.5 * 2^23 (two full-rate instructions; the conversion instruction runs at an
-// eighth of their rate and would bound layers of small K).
 template <typename T, bool SMALLK>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
@@ -470,13 +407,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
           const ulonglong2 s4 = sq[j / 4];
 #pragma unroll
           for (int h = 0; h < 4; h += 2) {
-            uint64_t a;
-            if (SMALLK)
-              a = add2(pk(__uint_as_float(v[j + h] + 0x4B400000u),
-                          __uint_as_float(v[j + h + 1] + 0x4B400000u)),
-                       pk(-12582912.f, -12582912.f));
-            else
-              a = pk((float)(int)v[j + h], (float)(int)v[j + h + 1]);
+            const uint64_t a = sums2<SMALLK>(v[j + h], v[j + h + 1]);
             upk(fma2(mul2(a, h ? s4.y : s4.x), sw2, b2), f[j + h], f[j + h + 1]);
           }
         }
@@ -540,8 +471,263 @@ int product(const void *xq, const void *wq, LinParams p, int K, int pitch, cudaS
     }
   }
   p.tiles = p.tiles_n * ((p.rows + p.bt - 1) / p.bt);
-  return K <= 260 ? launch_product<T, true>(xq, wq, p, pitch, st)  // 127^2 K < 2^22
-                  : launch_product<T, false>(xq, wq, p, pitch, st);
+  return K <= kSmallK ? launch_product<T, true>(xq, wq, p, pitch, st)
+                      : launch_product<T, false>(xq, wq, p, pitch, st);
+}
+
+// ---------------------------------------------------------------- few tokens --
+// The same product for few tokens, whose quantiser is part of it: every CTA
+// makes the codes of all of them itself, in the layout of the MMA operand, while
+// its first weights arrive. Up to 32768 elements of x that takes under a
+// microsecond, less than a launch of its own (80 x 128 x 384 and 1 x 512 x 18385:
+// one launch and no scratch memory instead of two and some).
+constexpr int kFewTokens = 128, kFewElements = 32768, kFewCodes = 64 * 1024, kFewStages = 8;
+
+bool is_few(long long rows, int K) {
+  if (rows > kFewTokens || rows * K > kFewElements) return false;
+  const int bt = (int)(rows + kUnit - 1) / kUnit * kUnit;
+  return (K + 127) / 128 * bt * 128 <= kFewCodes;
+}
+
+constexpr int kFewOffSx = 0;                                      // [kFewTokens]
+constexpr int kFewOffBar = kFewOffSx + kFewTokens * 4;
+constexpr int kFewOffMisc = kFewOffBar + (2 * kFewStages + 5) * 8;
+constexpr int kFewOffCodes = (kFewOffMisc + 16 + 1023) / 1024 * 1024;  // [ksteps][bt][128]
+constexpr int few_smem(int ksteps, int bt, int stages) {
+  return kFewOffCodes + ksteps * bt * 128 + stages * kStageA + 1024;
+}
+
+struct FewParams {
+  LinParams lin;
+  const void *x;
+  int K;
+  bool vec;  // four elements of a row at a time
+};
+
+template <typename X>
+__device__ __forceinline__ void load4(float (&f)[4], const X *x, int k, int K, bool vec) {
+  if (vec) {
+    if constexpr (sizeof(X) == 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(x + k));
+      f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    } else {
+      const uint2 v = __ldg(reinterpret_cast<const uint2 *>(x + k));
+      const X *e = reinterpret_cast<const X *>(&v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = to_f32(e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = k + j < K ? to_f32(x[k + j]) : 0.f;
+  }
+}
+
+template <typename X, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_i8_few_kernel(const __grid_constant__ CUtensorMap wmap, const FewParams q) {
+  const LinParams &p = q.lin;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float *sx = reinterpret_cast<float *>(smem + kFewOffSx);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kFewOffBar);
+  uint64_t *empty = full + kFewStages;
+  uint64_t *acc_full = empty + kFewStages;  // [2]
+  uint64_t *acc_empty = acc_full + 2;       // [2]
+  uint64_t *codes_ready = acc_empty + 2;
+  uint32_t *s_tmem = reinterpret_cast<uint32_t *>(smem + kFewOffMisc);
+  volatile int *s_abort = reinterpret_cast<volatile int *>(smem + kFewOffMisc + 4);
+  const int KS = p.ksteps;
+  uint8_t *codes = smem + kFewOffCodes, *ring = codes + KS * p.bt * 128;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kFewStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], kEpiWarps);
+    }
+    mbar_init(codes_ready, kEpiWarps);
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(s_tmem, 2 * kFewTokens);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&wmap);
+      int s = 0, used = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (TileWalk t(p); ok && !t.done(); t.next()) {
+        for (int k = 0; k < KS; ++k) {
+          if (used == p.stages && !mbar_wait_bounded(&empty[s], phase ^ 1, s_abort, p.err, 85)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], kStageA);
+          tma_load_2d(ring + s * kStageA, &wmap, &full[s], 128 * k, t.ni * kBM);
+          if (used < p.stages) ++used;
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (*s_abort) {  // leave no copy in flight
+        for (int i = 0; i < used; ++i) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(&full[i], i < s ? phase : phase ^ 1))
+            if (clock64() - t0 > (1ll << 30)) break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = idesc_i8(kBM, p.bt);
+      const uint64_t wdesc = sw128_kmajor_desc(smem_u32(ring));
+      const uint64_t xdesc = sw128_kmajor_desc(smem_u32(codes));
+      int s = 0;
+      uint32_t phase = 0;
+      Ring<2> acc;
+      bool ok = mbar_wait_bounded(codes_ready, 0, s_abort, p.err, 86);
+      for (TileWalk t(p); ok && !t.done(); t.next()) {
+        if (!acc.first && !mbar_wait_bounded(&acc_empty[acc.i], acc.phase ^ 1, s_abort, p.err, 87))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc.i * kFewTokens;
+        for (int k = 0; k < KS; ++k) {
+          if (!mbar_wait_bounded(&full[s], phase, s_abort, p.err, 88)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t a = wdesc + (uint64_t)(s * kStageA >> 4);
+          const uint64_t b = xdesc + (uint64_t)(k * p.bt * 128 >> 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mma_i8(d, a + 2 * i, b + 2 * i, idesc, k > 0 || i > 0 ? 1u : 0u);
+          mma_commit(&empty[s]);
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+        mma_commit(&acc_full[acc.i]);
+        acc.next();
+      }
+    }
+  } else {
+    const int ew = warp - kEpiWarp0;
+    // codes: a warp per row; what lies behind K or behind the last row meets
+    // weights of zero, or is not stored
+    for (int r = ew; r < (int)p.rows; r += kEpiWarps) {
+      const X *xr = static_cast<const X *>(q.x) + (size_t)r * q.K;
+      uint32_t top = 0;
+#pragma unroll 4
+      for (int k = 4 * lane; k < q.K; k += 128) {
+        float f[4];
+        load4(f, xr, k, q.K, q.vec);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+      }
+      const float big = __uint_as_float(__reduce_max_sync(~0u, top));
+      const bool finite = big < INFINITY;
+      const float s = finite ? fmaxf(big / 127.f, 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
+      const float inv = 1.f / s;
+      if (lane == 0) sx[r] = s;
+#pragma unroll 4
+      for (int k = 4 * lane; k < q.K; k += 128) {
+        float f[4];
+        load4(f, xr, k, q.K, q.vec);
+        // 128-byte swizzle: 16-byte pieces of a row change places by row mod 8
+        *reinterpret_cast<uint32_t *>(codes + (k >> 7) * p.bt * 128 + r * 128 +
+                                      ((k & 127) ^ ((r & 7) << 4))) =
+            finite ? codes4(f, s, inv) : 0u;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(codes_ready);
+    // every warp needs every row's scale
+    const bool ready = mbar_wait_bounded(codes_ready, 0, s_abort, p.err, 89);
+
+    const int g = ew >> 2;      // takes units g, g + 4, ... of the tokens
+    const int quad = warp & 3;  // the TMEM lanes a warp may read
+    const uint32_t tl = tmem + ((uint32_t)(quad * 32) << 16);
+    const int units = p.bt / kUnit;
+    Ring<2> acc;
+    for (TileWalk t(p); ready && !t.done(); t.next(), acc.next()) {
+      const int n = t.ni * kBM + quad * 32 + lane;
+      const float sw = n < p.N ? __ldg(p.sw + n) : 0.f;
+      const float b = n < p.N && p.bias ? __ldg(p.bias + n) : 0.f;
+      if (!mbar_wait_bounded(&acc_full[acc.i], acc.phase, s_abort, p.err, 90)) break;
+      tc_fence_after();
+      for (int u = g; u < units; u += 4) {
+        uint32_t v[kUnit];
+        tmem_ld16(tl + acc.i * kFewTokens + u * kUnit, v);
+        tmem_ld_wait(v);
+        float f[kUnit];
+#pragma unroll
+        for (int j = 0; j < kUnit; ++j) {
+          f[j] = fmaf((float)(int)v[j] * sx[u * kUnit + j], sw, b);
+          if (p.act) f[j] = activate(f[j], p.act);
+        }
+        if (n < p.N) {
+          T *o = static_cast<T *>(p.y) + (long long)u * kUnit * p.N + n;
+          store_unit<T, false>(o, p.N, f, (int)p.rows - u * kUnit);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc.i]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * kFewTokens);
+  }
+}
+
+template <typename X, typename T>
+int launch_few(FewParams q, const void *wq, int pitch, cudaStream_t st) {
+  LinParams &p = q.lin;
+  CUtensorMap wm;
+  int rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, pitch, p.N, pitch, kBM);
+  if (rc) return rc;
+  q.vec = q.K % 4 == 0 && aligned(q.x, 4 * sizeof(X));
+  p.bt = (int)(p.rows + kUnit - 1) / kUnit * kUnit;
+  p.tiles_n = (p.N + kBM - 1) / kBM;
+  p.tiles = p.tiles_n;
+  const int grid = (int)(p.tiles < sm_count() ? p.tiles : sm_count());
+  const long long steps = (p.tiles + grid - 1) / grid * p.ksteps;
+  p.stages = steps < kFewStages ? (int)steps : kFewStages;
+  auto *kernel = linear_i8_few_kernel<X, T>;
+  constexpr int most = kFewOffCodes + kFewCodes + kFewStages * kStageA + 1024;
+  static_assert(most <= 227 * 1024, "shared memory");
+  rc = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), most, "linear_i8_few_kernel");
+  if (rc) return rc;
+  kernel<<<grid, kThreads, few_smem(p.ksteps, p.bt, p.stages), st>>>(wm, q);
+  return check_launch("linear_i8_few_kernel");
+}
+
+template <typename X>
+int few(const FewParams &q, const void *wq, int pitch, int out_dtype, cudaStream_t st) {
+  if (out_dtype == TOCR_DTYPE_F16) return launch_few<X, __half>(q, wq, pitch, st);
+  if (out_dtype == TOCR_DTYPE_BF16) return launch_few<X, __nv_bfloat16>(q, wq, pitch, st);
+  return launch_few<X, float>(q, wq, pitch, st);
 }
 
 constexpr long long kMaxRows = 1ll << 24;
@@ -561,11 +747,9 @@ int check_linear(const char *fn, long long rows, int K, int N, int act, int out_
   return TOCR_OK;
 }
 
-int run_product(const void *xq, const float *sx, long long rows, int K, const void *wq,
-                const float *sw, const float *bias, int N, int act, int out_dtype, void *y,
-                int *err, bool behind_quant, cudaStream_t st) {
+LinParams params(const float *sx, long long rows, int K, const float *sw, const float *bias, int N,
+                 int act, void *y, int *err) {
   LinParams p{};
-  p.behind_quant = behind_quant;
   p.sx = sx;
   p.sw = sw;
   p.bias = bias;
@@ -575,12 +759,20 @@ int run_product(const void *xq, const float *sx, long long rows, int K, const vo
   p.ksteps = (K + 127) / 128;
   p.act = act;
   p.err = err;
+  return p;
+}
+
+int run_product(const void *xq, const void *wq, const LinParams &p, int K, int out_dtype,
+                cudaStream_t st) {
   const int pitch = (K + 15) / 16 * 16;
+  if (wants_row_kernel(p.y, p.rows, p.N, out_dtype == TOCR_DTYPE_F32 ? 4 : 2))
+    return launch_row_kernel(xq, wq, p, K, pitch, out_dtype, st);
   if (out_dtype == TOCR_DTYPE_F16) return product<__half>(xq, wq, p, K, pitch, st);
   if (out_dtype == TOCR_DTYPE_BF16) return product<__nv_bfloat16>(xq, wq, p, K, pitch, st);
   return product<float>(xq, wq, p, K, pitch, st);
 }
 
+// the codes of a call's tokens; its scales lie behind them
 size_t codes_bytes(long long rows, int K) {
   return ((size_t)rows * ((K + 15) / 16 * 16) + 255) / 256 * 256;
 }
@@ -618,12 +810,12 @@ TOCR_API int tocr_linear_i8_codes(const void *d_xq, const float *d_sx, long long
                "tocr_linear_i8_codes: the codes must be 16-byte aligned");
   TOCR_REQUIRE(aligned(d_y, out_dtype == TOCR_DTYPE_F32 ? 4 : 2),
                "tocr_linear_i8_codes: y must be aligned to its element");
-  return run_product(d_xq, d_sx, rows, K, d_wq, d_sw, d_bias, N, act, out_dtype, d_y, d_err,
-                     false, as_stream(stream));
+  return run_product(d_xq, d_wq, params(d_sx, rows, K, d_sw, d_bias, N, act, d_y, d_err), K,
+                     out_dtype, as_stream(stream));
 }
 
 TOCR_API size_t tocr_linear_i8_workspace_bytes(long long rows, int K) {
-  if (rows < 0 || rows > kMaxRows || K <= 0 || K > kMaxK) return 0;
+  if (rows < 0 || rows > kMaxRows || K <= 0 || K > kMaxK || is_few(rows, K)) return 0;
   return codes_bytes(rows, K) + (size_t)rows * 4;
 }
 
@@ -636,21 +828,30 @@ TOCR_API int tocr_linear_i8(const void *d_x, int x_dtype, long long rows, int K,
   if (rc) return rc;
   TOCR_REQUIRE(is_dtype(x_dtype), "tocr_linear_i8: unknown type %d", x_dtype);
   if (rows == 0) return TOCR_OK;
-  TOCR_REQUIRE(d_x && d_wq && d_sw && d_y && d_workspace && d_err, "tocr_linear_i8: null pointer");
+  TOCR_REQUIRE(d_x && d_wq && d_sw && d_y && d_err, "tocr_linear_i8: null pointer");
   TOCR_REQUIRE(aligned(d_wq, 16), "tocr_linear_i8: the codes must be 16-byte aligned");
   TOCR_REQUIRE(aligned(d_x, x_dtype == TOCR_DTYPE_F32 ? 4 : 2) &&
                    aligned(d_y, out_dtype == TOCR_DTYPE_F32 ? 4 : 2),
                "tocr_linear_i8: x and y must be aligned to their elements");
-  TOCR_REQUIRE(aligned(d_workspace, 256) && workspace_bytes >= codes_bytes(rows, K) + (size_t)rows * 4,
-               "tocr_linear_i8: the workspace must be 256-byte aligned and hold %zu bytes",
-               codes_bytes(rows, K) + (size_t)rows * 4);
   cudaStream_t st = as_stream(stream);
+  LinParams p = params(nullptr, rows, K, d_sw, d_bias, N, act, d_y, d_err);
+  if (is_few(rows, K)) {
+    const FewParams q = {p, d_x, K, false};
+    const int pitch = (K + 15) / 16 * 16;
+    if (x_dtype == TOCR_DTYPE_F16) return few<__half>(q, d_wq, pitch, out_dtype, st);
+    if (x_dtype == TOCR_DTYPE_BF16) return few<__nv_bfloat16>(q, d_wq, pitch, out_dtype, st);
+    return few<float>(q, d_wq, pitch, out_dtype, st);
+  }
+  const size_t need = codes_bytes(rows, K) + (size_t)rows * 4;
+  TOCR_REQUIRE(d_workspace && aligned(d_workspace, 256) && workspace_bytes >= need,
+               "tocr_linear_i8: the workspace must be 256-byte aligned and hold %zu bytes", need);
   int8_t *q = static_cast<int8_t *>(d_workspace);
   float *sx = reinterpret_cast<float *>(q + codes_bytes(rows, K));
   rc = quant_rows(d_x, x_dtype, rows, K, q, sx, st);
   if (rc) return rc;
-  return run_product(q, sx, rows, K, d_wq, d_sw, d_bias, N, act, out_dtype, d_y, d_err,
-                     true, st);
+  p.sx = sx;
+  p.behind_quant = true;
+  return run_product(q, d_wq, p, K, out_dtype, st);
 }
 
 }  // extern "C"

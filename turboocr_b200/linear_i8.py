@@ -86,9 +86,9 @@ def linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias: torch.Tens
     def launch(s):
         y = torch.empty(rows, N, dtype=out_dtype, device=x.device)
         n = lib().tocr_linear_i8_workspace_bytes(rows, K)
-        buf = torch.empty(n, dtype=torch.uint8, device=x.device)
-        call("tocr_linear_i8", px, DTYPES[x.dtype], rows, K, *w, y.data_ptr(), buf.data_ptr(), n,
-             pe, s)
+        buf = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        call("tocr_linear_i8", px, DTYPES[x.dtype], rows, K, *w, y.data_ptr(),
+             buf.data_ptr() if n else None, n, pe, s)
         return y
 
     return on(dev, stream, launch)
