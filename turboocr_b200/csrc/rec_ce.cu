@@ -733,55 +733,50 @@ __device__ __forceinline__ float warp_dot(const uint8_t *a, const uint8_t *b, in
   return s;
 }
 
-// Joins the pieces of every kept row, in the order of the vocabulary: a CTA
-// takes 32 rows of a tile, eight threads per row a run of its pieces each. The
-// target's logit is a dot product here: picking it out of the tiles would cost
-// every tile a search.
+// Joins the pieces of every kept row, a warp per row: lane c takes pieces c, c +
+// 32, ... (a fixed order). The target's logit is a dot product here: picking it
+// out of the tiles would cost every tile a search.
 template <bool BF16>
 __global__ void __launch_bounds__(256)
 ce_loss_kernel(const FwdParams p, const uint8_t *w, const float *bias, const int *tgt, int grid,
                float *loss, float *lse) {
   __shared__ int s_first, s_last;
-  __shared__ float2 s_run[8][32];
-  __shared__ float s_lt[32];
   after_previous();
   const int n = p.hdr->n;
-  const int tile = blockIdx.x / (kTile / 32), r0 = blockIdx.x % (kTile / 32) * 32;
-  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
-  const int row0 = tile * kTile + r0;
-  if (row0 >= n) return;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int tile = blockIdx.x * 8 / kTile;
+  if ((int)blockIdx.x * 8 >= n) return;
   if (threadIdx.x == 0) {
     const Cuts cuts((long long)((n + kTile - 1) / kTile) * p.chunks, grid);
     s_first = cuts.owner((long long)tile * p.chunks);
     s_last = cuts.owner((long long)(tile + 1) * p.chunks - 1);
   }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int row = row0 + run * 4 + k;
-    if (row >= n) break;
-    const int t = tgt[row];
-    const float d = warp_dot<BF16>(p.feat + (size_t)p.rowidx[row] * p.K * 2,
-                                   w + (size_t)t * p.K * 2, p.K, lane);
-    if (lane == 0) s_lt[run * 4 + k] = d + (bias ? bias[t] : 0.f);
-  }
+  const bool live = row < n;
+  const int i = live ? p.rowidx[row] : 0, t = live ? tgt[row] : 0;
+  const float b = live && bias ? bias[t] : 0.f;
+  const float lt =
+      live ? warp_dot<BF16>(p.feat + (size_t)i * p.K * 2, w + (size_t)t * p.K * 2, p.K, lane) : 0.f;
   __syncthreads();
-  const int pieces = s_last - s_first + 1, per = (pieces + 7) / 8;
-  float M = -INFINITY, S = 0.f;
-  auto join = [&](float2 v) {  // a NaN shows in the sums only
+  if (!live) return;
+  const int pieces = s_last - s_first + 1;
+  const float2 *src = p.part + (size_t)(tile + s_first) * kTile + row % kTile;
+  float M = -INFINITY, S = 0.f;  // a NaN shows in the sums only
+#pragma unroll 4
+  for (int c = lane; c < pieces; c += 32) {
+    const float2 v = src[(size_t)c * kTile];
     const float m = fmaxf(M, v.x);
     S = (M == -INFINITY ? S : S * exp2f(M - m)) + (v.x == -INFINITY ? v.y : v.y * exp2f(v.x - m));
     M = m;
-  };
-  const float2 *src = p.part + (size_t)(tile + s_first) * kTile + r0 + lane;
-#pragma unroll 4
-  for (int c = run * per; c < min(pieces, (run + 1) * per); ++c) join(src[(size_t)c * kTile]);
-  s_run[run][lane] = make_float2(M, S);
-  __syncthreads();
-  if (run > 0 || row0 + lane >= n) return;
-  for (int k = 1; k < 8; ++k) join(s_run[k][lane]);
-  const float z = fmaf(M, kLn2, logf(S));
-  const float l = z - s_lt[lane];
-  const int i = p.rowidx[row0 + lane];
+  }
+  float top = M;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  if (M != -INFINITY) S *= exp2f(M - top);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(~0u, S, o);
+  if (lane > 0) return;
+  const float z = fmaf(top, kLn2, logf(S));
+  const float l = z - (lt + b);
   lse[i] = z;
   loss[i] = l < 0.f ? 0.f : l;  // a sum is its own term at least; keeps NaN
 }
@@ -1211,7 +1206,7 @@ ce_join_kernel(const BwdParams p, int cn, int KP, int grid) {
       if (k >= p.K) continue;
       const float *src = p.dpart + (size_t)r * KP + k;
       float4 s = *reinterpret_cast<const float4 *>(src + (size_t)(2 * c - 1) * ps);
-#pragma unroll 4
+#pragma unroll 8
       for (int d = c; d <= last; ++d) {
         const float4 v = *reinterpret_cast<const float4 *>(src + 2 * (size_t)d * ps);
         s.x += v.x;
@@ -1311,10 +1306,12 @@ int launch_place(const Workspace &ws, const void *targets, bool wide, int rows, 
   p.nlse = ws.nlse;
   p.gc = ws.gc;
   p.gs = ws.gs;
+  // shares enough for one or two passes over the bias, 8 for the copies
+  const int per = (V + blocks * kRowBlock - 1) / (blocks * kRowBlock);
+  const dim3 shares(blocks, per < 8 ? 8 : per < 64 ? per : 64);
   if (!direct)
-    return launch_overlapped("ce_place_kernel", ce_place_kernel<BWD>, dim3(blocks, 8), kRowBlock, 0,
-                             st, p);
-  ce_place_kernel<BWD><<<dim3(blocks, 8), kRowBlock, 0, st>>>(p);
+    return launch_overlapped("ce_place_kernel", ce_place_kernel<BWD>, shares, kRowBlock, 0, st, p);
+  ce_place_kernel<BWD><<<shares, kRowBlock, 0, st>>>(p);
   return check_launch("ce_place_kernel");
 }
 
@@ -1383,7 +1380,7 @@ TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *
   }
   if (rc) return rc;
   return launch_overlapped("ce_loss_kernel", bf ? ce_loss_kernel<true> : ce_loss_kernel<false>,
-                           tiles * (kTile / 32), 256, 0, st, p, static_cast<const uint8_t *>(d_w),
+                           tiles * (kTile / 8), 256, 0, st, p, static_cast<const uint8_t *>(d_w),
                            d_bias, ws.tgt, grid, d_loss, d_lse);
 }
 
@@ -1439,7 +1436,8 @@ TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, cons
   p.err = d_err;
   const long long tiles_x = p.want_x ? (rows + kTile - 1) / kTile : 0;
   const long long chunks_r = rows > cn ? (rows + cn - 1) / cn : 1;
-  const int grid = grid_for(tiles_x * p.chunks_v + p.tiles_w * chunks_r, 1);
+  // two steps at least: fewer pieces to join (175 x 64 x 5000: 80 CTAs and not 148)
+  const int grid = grid_for(tiles_x * p.chunks_v + p.tiles_w * chunks_r, 2);
   const int rows_pad = (int)((rows + kTile - 1) / kTile * kTile + kTile);
   const bool bf = dtype == TOCR_DTYPE_BF16;
   switch (KA) {
