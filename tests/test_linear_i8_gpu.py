@@ -117,3 +117,106 @@ def test_output_at_any_element_and_nothing_written_around_it(tocr, cuda, rows, N
         assert torch.equal(buf[pad + off:pad + off + rows * N].view(rows, N), want), off
         assert bool((buf[:pad + off] == -7).all()) and bool((buf[pad + off + rows * N:] == -7).all())
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("rows", [5, 600])   # few tokens and many take different kernels
+@pytest.mark.parametrize("xt", [F16, BF16, F32])
+def test_rows_of_any_numbers(tocr, cuda, rows, xt):
+    """Zero rows, rows of the least and the largest numbers, rows whose quotients
+    are ties, and rows with an infinity or a NaN (NaN outputs, the others as
+    without them)."""
+    K, N = 96, 130
+    g = torch.Generator(device="cpu").manual_seed(rows)
+    x = torch.randn(rows, K, generator=g).to(xt)
+    x[0] = 0
+    x[1] = torch.finfo(xt).smallest_normal * torch.finfo(xt).eps * torch.randint(-9, 10, (K,)).to(xt)
+    x[2] = torch.finfo(xt).max * (torch.rand(K, generator=g) * 2 - 1).to(xt)
+    x[3] = torch.arange(K).to(xt) / 2           # half of the maximum is a tie
+    x[4] = (torch.arange(K) % 3 - 1).to(xt) * 12.7
+    w = (torch.randn(N, K, generator=g) / math.sqrt(K)).to(cuda)
+    w[7] = 0
+    bias = torch.randn(N, generator=g).to(cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    x = x.to(cuda)
+    check(x[torch.arange(rows) != 2].contiguous(), w, bias, "none", F32, err)
+    y = check(x, w * 1e-3, bias, "none", F32, err)
+    assert torch.equal(y[0], bias)
+    bad = x.clone()
+    bad[1, 5], bad[4, 95] = math.inf, math.nan
+    wq, ws = linear_i8.quantize_rows(w * 1e-3)
+    codes, scales = linear_i8.quantize_rows(bad)
+    assert bool(torch.isnan(scales[[1, 4]]).all()) and int(codes[[1, 4]].abs().sum()) == 0
+    for act in ("none", "relu", "hardswish"):
+        z = linear_i8.linear(bad, wq, ws, bias, act=act, out_dtype=F32, err=err)
+        ref = linear_i8.linear(x, wq, ws, bias, act=act, out_dtype=F32, err=err)
+        assert bool(torch.isnan(z[[1, 4]]).all())
+        rest = [r for r in range(rows) if r not in (1, 4)]
+        assert torch.equal(z[rest], ref[rest])
+    assert int(err) == 0
+
+
+def test_weights_with_a_nan_channel(tocr, cuda):
+    w = torch.randn(40, 64, device=cuda)
+    w[3, 3] = math.nan
+    wq, ws = linear_i8.quantize_rows(w)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    for rows in (3, 700):
+        y = linear_i8.linear(torch.randn(rows, 64, device=cuda), wq, ws, None, err=err)
+        assert bool(torch.isnan(y[:, 3]).all())
+        assert bool(torch.isfinite(y[:, :3]).all()) and bool(torch.isfinite(y[:, 4:]).all())
+
+
+def test_few_tokens_border(tocr, cuda):
+    """Sizes at both sides of the rule that has the product quantise its tokens."""
+    g = torch.Generator(device="cpu").manual_seed(2)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    for rows, K, N in ((128, 256, 300), (129, 250, 300), (128, 257, 300), (17, 1900, 5),
+                       (16, 2048, 20000), (8, 4096, 129), (1, 4097, 128), (1, 32768, 40),
+                       (1, 40000, 40), (3, 13, 19000)):
+        x = torch.randn(rows, K, generator=g).to(BF16).to(cuda)
+        w = (torch.randn(N, K, generator=g) / math.sqrt(K)).to(cuda)
+        check(x, w, None, "relu", BF16, err)
+
+
+def test_empty_and_other_streams_and_graphs(tocr, cuda):
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    w = torch.randn(500, 200, device=cuda)
+    wq, ws = linear_i8.quantize_rows(w)
+    assert linear_i8.linear(torch.zeros(0, 200, device=cuda), wq, ws, err=err).shape == (0, 500)
+    assert linear_i8.quantize_rows(torch.zeros(0, 200, device=cuda))[0].shape == (0, 208)
+    xs = [torch.randn(r, 200, device=cuda, dtype=F16) for r in (3, 900)]
+    want = [linear_i8.linear(x, wq, ws, err=err) for x in xs]
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = [linear_i8.linear(x, wq, ws, err=err, stream=s) for _ in range(8)
+           for x, s in zip(xs, (s1, s2))]
+    torch.cuda.synchronize()
+    for k, y in enumerate(got):
+        assert torch.equal(y, want[k % 2])
+    held = [x.clone() for x in xs]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = [linear_i8.linear(x, wq, ws, err=err) for x in held]
+    for x in held:
+        x.mul_(0.5)
+    g.replay()
+    torch.cuda.synchronize()
+    for x, y in zip(held, out):
+        assert torch.equal(y, linear_i8.linear(x, wq, ws, err=err))
+    assert int(err) == 0
+
+
+def test_output_beyond_32_bits(tocr, cuda):
+    rows, K, N = 120001, 32, 18385             # 4.4 GB of fp16
+    g = torch.Generator(device=cuda).manual_seed(4)
+    x = torch.randn(rows, K, generator=g, device=cuda, dtype=F16)
+    wq, ws = linear_i8.quantize_rows(torch.randn(N, K, generator=g, device=cuda))
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    y = linear_i8.linear(x, wq, ws, None, err=err)
+    for at in (slice(0, 300), slice(116700, 117000), slice(rows - 300, rows)):
+        part = linear_i8.linear(x[at].contiguous(), wq, ws, None, err=err)
+        assert torch.equal(y[at], part)
+    y = linear_i8.linear(x, wq[:18368].contiguous(), ws[:18368].contiguous(), None, err=err)
+    assert torch.equal(y[-300:], linear_i8.linear(x[-300:].contiguous(), wq, ws, None,
+                                                  err=err)[:, :18368])
+    assert int(err) == 0

@@ -8,7 +8,9 @@
 //
 // the numerics that tocr_dwpw_block uses per pixel, for the recognizer's
 // linear layers. The sum is exact in s32 (K up to 131072); the epilogue is
-// fp32 and rounds once to the output type. A row that holds an infinity or a
+// fp32, the channel's scale first (weights are of ordinary size, so neither the
+// largest nor the least activations leave fp32's range on the way), and rounds
+// once to the output type. A row that holds an infinity or a
 // NaN gets the scale NaN, so its outputs are NaN instead of silently wrong.
 //
 // Quantiser: one pass over x from memory (a row's values stay in registers
@@ -408,7 +410,7 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
 #pragma unroll
           for (int h = 0; h < 4; h += 2) {
             const uint64_t a = sums2<SMALLK>(v[j + h], v[j + h + 1]);
-            upk(fma2(mul2(a, h ? s4.y : s4.x), sw2, b2), f[j + h], f[j + h + 1]);
+            upk(fma2(mul2(a, sw2), h ? s4.y : s4.x, b2), f[j + h], f[j + h + 1]);
           }
         }
         if (p.act) {
@@ -680,7 +682,7 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap wmap, const FewParams q
         float f[kUnit];
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
-          f[j] = fmaf((float)(int)v[j] * sx[u * kUnit + j], sw, b);
+          f[j] = fmaf((float)(int)v[j] * sw, sx[u * kUnit + j], b);
           if (p.act) f[j] = activate(f[j], p.act);
         }
         if (n < p.N) {

@@ -302,7 +302,7 @@ linear_i8_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
           for (int h = 0; h < 2; ++h) {
             const uint32_t *q = &w[i >> 1][4 * h + 2 * (i & 1)];
             const uint64_t a = sums2<SMALLK>(q[0], q[1]);
-            upk(fma2(mul2(a, sx2[i]), sb[h].x, sb[h].y), f[i][h][0], f[i][h][1]);
+            upk(fma2(mul2(a, sb[h].x), sx2[i], sb[h].y), f[i][h][0], f[i][h][1]);
           }
         if (p.act) {
 #pragma unroll
