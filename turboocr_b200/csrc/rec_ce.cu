@@ -84,12 +84,13 @@ struct Workspace {
   float *gblk;
   int *rowidx;     // [rows_pad] the row of each kept row
   int *tgt;        // [rows_pad] its target (-1 behind the last)
-  float *bias2;    // [V to 128] bias * log2(e), -inf behind the last class
+  float *bias2;    // [V to 128] bias * log2(e) (backward: + log2 of P's scale), -inf behind the last
   // forward
+  float *lt;       // [rows_pad] the target's logit
   float2 *part;    // [tiles + grid][128] (base, sum) of a range's piece of a tile
   // backward
   uint8_t *xc;     // [rows_pad][K] the kept rows of F, zero behind the last
-  float *nlse;     // [rows_pad] -lse * log2(e) (-inf behind the last)
+  float *nlse;     // [rows_pad] -lse (-inf behind the last)
   float *gc;       // [rows_pad] g
   float *gs;       // [rows_pad] g / gmax * 2^shift
   float *dpart;    // [2 * grid][128][KP]
@@ -117,6 +118,7 @@ inline Workspace carve(uint8_t *base, long long rows, int K, int V, bool backwar
   w.tgt = reinterpret_cast<int *>(take(pad * 4));
   w.bias2 = reinterpret_cast<float *>(take(((size_t)V + 127) / 128 * 128 * 4));
   if (!backward) {
+    w.lt = reinterpret_cast<float *>(take(pad * 4));
     w.part = reinterpret_cast<float2 *>(take((size_t)(pad / kTile + grid) * kTile * 8));
   } else {
     w.xc = take((size_t)pad * K * 2);
@@ -167,7 +169,8 @@ struct PlaceParams {
   const void *targets;
   bool wide;
   int rows, V, K;
-  float shift;       // 2^14 for fp16, 1 for bf16
+  float shift;       // scale of P: 2^14 for fp16, 1 for bf16
+  float shift2;      // its log2
   bool direct;       // no cnt, gblk: count here
   const int *cnt;
   const float *gblk;
@@ -248,14 +251,14 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
   const bool share0 = blockIdx.y == 0;
   for (int v = (blockIdx.y * gridDim.x + blockIdx.x) * kRowBlock + tid; v < (p.V + 127) / 128 * 128;
        v += gridDim.x * gridDim.y * kRowBlock)
-    p.bias2[v] = v < p.V ? (p.bias ? p.bias[v] * kLog2e : 0.f) : -INFINITY;
+    p.bias2[v] = v < p.V ? (p.bias ? p.bias[v] * kLog2e : 0.f) + (BWD ? p.shift2 : 0.f) : -INFINITY;
   if (share0 && i < p.rows) {
     if (t >= 0) {
       p.rowidx[dst] = (int)i;
       p.tgt[dst] = t;
       if (BWD) {
         const float g = p.g[i];
-        p.nlse[dst] = -p.lse[i] * kLog2e;
+        p.nlse[dst] = -p.lse[i];
         p.gc[dst] = g;
         p.gs[dst] = s_gmax > 0.f ? g / s_gmax * p.shift : g * 0.f;
       }
@@ -339,7 +342,7 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return r;
 }
 
-// y = l * log2(e) + terms of 32 columns, in pairs
+// y = S * log2(e) + terms of 32 columns, in pairs
 __device__ __forceinline__ void logits32(uint64_t (&y)[16], const uint32_t (&v)[32],
                                          const float *terms) {
   const uint64_t l2e2 = pk(kLog2e, kLog2e);
@@ -351,6 +354,15 @@ __device__ __forceinline__ void logits32(uint64_t (&y)[16], const uint32_t (&v)[
     y[2 * q + 1] =
         fma2(pk(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])), l2e2, c.y);
   }
+}
+// takes column `at` out of 32 (leaves -inf there)
+__device__ __forceinline__ void take_out(uint32_t (&v)[32], int at, float &taken) {
+#pragma unroll
+  for (int q = 0; q < 32; ++q)
+    if (at == q) {
+      taken = __uint_as_float(v[q]);
+      v[q] = 0xff800000u;
+    }
 }
 // exp2 of a pair without the special-function unit: y = n + f, |f| <= 1/2, by
 // adding and taking off 1.5 * 2^23; exp2(f) by its Taylor polynomial in f ln 2
@@ -383,7 +395,7 @@ __device__ __forceinline__ void add_exp(uint64_t (&s)[4], const uint64_t (&y)[16
 #pragma unroll
   for (int q = 0; q < 16; ++q) {
     const uint64_t z = BASE ? add2(y[q], nb) : y[q];
-    if (q % 16 < kPolyPairs) {
+    if (q < kPolyPairs) {
       s[q & 3] = add2(s[q & 3], ex2_poly(z));
     } else {
       float a, b;
@@ -451,9 +463,10 @@ struct FwdCfg {
 
 struct FwdParams {
   const uint8_t *feat;
-  const float *bias2;
+  const float *bias, *bias2;
   const Header *hdr;
-  const int *rowidx;
+  const int *rowidx, *tgt;
+  float *lt;
   float2 *part;
   int V, K, chunks;
   int *err;
@@ -584,17 +597,19 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
       const int cnt = (int)min((long long)(NC - c0), it1 - it);
       const int row = tile * kTile + r;  // kept rows are numbered from 0
       const int src = row < n ? p.rowidx[row] : -1;
+      const int tg = row < n ? p.tgt[row] : -1;
       load_tile_tmem<KA>(tl + C::TX, src >= 0 ? p.feat + (size_t)src * p.K * 2 : nullptr, p.K,
                          ew >> 2);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(x_ready);
-      // sum of exp2(y - base), y = l * log2(e). The base is 0 if the first
-      // logits that the thread sees have their maximum within 2^64 of it, else
-      // that maximum: the sum cannot vanish. It grows with 64 logits whose sum
-      // passes 2^100, so it cannot overflow either, and no maximum is taken of
-      // the others.
+      // sum of exp2(y - base), y = l * log2(e), over the classes but the target
+      // (whose logit is kept aside, so that a well recognised row has an exact
+      // lse). The base is 0 if the first logits that the thread sees have their
+      // maximum within 2^64 of it, else that maximum: the sum cannot vanish. It
+      // grows with 64 logits whose sum passes 2^100, so it cannot overflow either,
+      // and no maximum is taken of the others.
       float sum = 0.f, base = 0.f;
       bool seen = false;               // this lane has its base
       bool fresh = true, based = false;  // some lane of the warp has none; one other than 0
@@ -607,10 +622,12 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
         tc_fence_after();
         const uint32_t ts = tl + C::TS + b * C::CN + half * 64;
         const float *terms = scol + cs * C::CN + half * 64;
-        float add = 0.f;
+        const int at = tg - ((c0 + i) * C::CN + half * 64);
+        const bool hit = __any_sync(~0u, at >= 0 && at < 64);
+        float add = 0.f, st = 0.f;  // st: S of the target
         bool slow = fresh;
-        if (!slow) {
-          const uint64_t nb = pk(-base, -base);
+        const uint64_t nb = pk(-base, -base);
+        if (!slow && !hit) {
           uint64_t s4[4] = {0, 0, 0, 0}, y[16];
           uint32_t v[32], w[32];
           tmem_ld32(ts, v);
@@ -628,8 +645,21 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
           else
             add_exp<false>(s4, y, nb);
           add = sum4(s4);
-          slow = __any_sync(~0u, !(add < 0x1p100f));
+        } else if (!slow) {  // one chunk in nine (18385 classes): without the targets
+          uint64_t s4[4] = {0, 0, 0, 0};
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g) {
+            uint32_t v[32];
+            uint64_t y[16];
+            tmem_ld32(ts + 32 * g, v);
+            tmem_ld_wait(v);
+            take_out(v, at - 32 * g, st);
+            logits32(y, v, terms + 32 * g);
+            add_exp<true>(s4, y, nb);
+          }
+          add = sum4(s4);
         }
+        slow = slow || __any_sync(~0u, !(add < 0x1p100f));
         if (slow) {  // a first or a larger base
           float gm = -INFINITY;
 #pragma unroll 1
@@ -638,6 +668,7 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
             uint64_t y[16];
             tmem_ld32(ts + 32 * g, v);
             tmem_ld_wait(v);
+            take_out(v, at - 32 * g, st);
             logits32(y, v, terms + 32 * g);
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
@@ -655,7 +686,7 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
           }
           fresh = __any_sync(~0u, !seen);
           based = __any_sync(~0u, base != 0.f);
-          const uint64_t nb = pk(-base, -base);
+          const uint64_t nb2 = pk(-base, -base);
           uint64_t s4[4] = {0, 0, 0, 0};
 #pragma unroll 1
           for (int g = 0; g < 2; ++g) {
@@ -663,11 +694,13 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
             uint64_t y[16];
             tmem_ld32(ts + 32 * g, v);
             tmem_ld_wait(v);
+            take_out(v, at - 32 * g, st);
             logits32(y, v, terms + 32 * g);
-            add_exp<true>(s4, y, nb);
+            add_exp<true>(s4, y, nb2);
           }
           add = sum4(s4);
         }
+        if (at >= 0 && at < 64) p.lt[row] = st + (p.bias ? p.bias[tg] : 0.f);
         sum += add;
         tc_fence_before();
         __syncwarp();
@@ -707,39 +740,13 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
   }
 }
 
-// sum of products of two rows of K 16-bit numbers, over the lanes of a warp
-template <bool BF16>
-__device__ __forceinline__ float warp_dot(const uint8_t *a, const uint8_t *b, int K, int lane) {
-  float s = 0.f;
-  if (8 * lane < K) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(a) + lane);
-    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(b) + lane);
-    const uint32_t x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float2 f, g;
-      if (BF16) {
-        f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&x[k]));
-        g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&y[k]));
-      } else {
-        f = __half22float2(*reinterpret_cast<const __half2 *>(&x[k]));
-        g = __half22float2(*reinterpret_cast<const __half2 *>(&y[k]));
-      }
-      s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
-    }
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  return s;
-}
-
 // Joins the pieces of every kept row, a warp per row: lane c takes pieces c, c +
-// 32, ... (a fixed order). The target's logit is a dot product here: picking it
-// out of the tiles would cost every tile a search.
-template <bool BF16>
+// 32, ... (a fixed order). With r = log sum exp of the other classes and l the
+// target's logit, lse = max(r, l) + log(1 + exp(-|r - l|)): exactly l where the
+// others do not count, so that the loss is exactly 0 and the backward pass finds
+// a probability of exactly 1.
 __global__ void __launch_bounds__(256)
-ce_loss_kernel(const FwdParams p, const uint8_t *w, const float *bias, const int *tgt, int grid,
-               float *loss, float *lse) {
+ce_loss_kernel(const FwdParams p, int grid, float *loss, float *lse) {
   __shared__ int s_first, s_last;
   after_previous();
   const int n = p.hdr->n;
@@ -751,13 +758,8 @@ ce_loss_kernel(const FwdParams p, const uint8_t *w, const float *bias, const int
     s_first = cuts.owner((long long)tile * p.chunks);
     s_last = cuts.owner((long long)(tile + 1) * p.chunks - 1);
   }
-  const bool live = row < n;
-  const int i = live ? p.rowidx[row] : 0, t = live ? tgt[row] : 0;
-  const float b = live && bias ? bias[t] : 0.f;
-  const float lt =
-      live ? warp_dot<BF16>(p.feat + (size_t)i * p.K * 2, w + (size_t)t * p.K * 2, p.K, lane) : 0.f;
   __syncthreads();
-  if (!live) return;
+  if (row >= n) return;
   const int pieces = s_last - s_first + 1;
   const float2 *src = p.part + (size_t)(tile + s_first) * kTile + row % kTile;
   float M = -INFINITY, S = 0.f;  // a NaN shows in the sums only
@@ -775,10 +777,11 @@ ce_loss_kernel(const FwdParams p, const uint8_t *w, const float *bias, const int
 #pragma unroll
   for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(~0u, S, o);
   if (lane > 0) return;
-  const float z = fmaf(top, kLn2, logf(S));
-  const float l = z - (lt + b);
+  const int i = p.rowidx[row];
+  const float l = p.lt[row], rest = fmaf(top, kLn2, logf(S));  // -inf without other classes
+  const float a = rest - l, z = (a > 0.f ? rest : l) + log1pf(expf(-fabsf(a)));
+  loss[i] = z - l;
   lse[i] = z;
-  loss[i] = l < 0.f ? 0.f : l;  // a sum is its own term at least; keeps NaN
 }
 
 // ------------------------------------------------------------- backward -----
@@ -803,7 +806,7 @@ struct BwdCfg {
 
 struct BwdParams {
   const uint8_t *w, *xc;
-  const float *bias2;
+  const float *bias, *bias2;
   const Header *hdr;
   const int *rowidx, *tgt;
   const float *nlse, *gc, *gs;
@@ -1020,11 +1023,14 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(x_ready);
-      // y = S * log2(e) + column term + row term; P = exp2(y) (* column scale)
+      // y = (S - lse) log2(e) + bias log2(e), P = exp2(y) (* column scale). The
+      // target's y is ((S + bias) - lse) log2(e), rounded as the forward pass
+      // rounds its logit: exactly 0 where the target alone counts.
       const int tg = !dw && real ? p.tgt[row] : -1;
-      float rterm = -INFINITY;
-      if (real) rterm = dw ? p.bias2[row] : p.nlse[row] + p.shift;
-      const uint64_t rt2 = pk(rterm, rterm);
+      const float bt = !p.bias ? 0.f : dw ? (real ? p.bias[row] : 0.f) : tg >= 0 ? p.bias[tg] : 0.f;
+      float rterm = -INFINITY;  // dF: -lse, dW: bias * log2(e)
+      if (real) rterm = dw ? bt * kLog2e : p.nlse[row];
+      const uint64_t rt2 = pk(rterm, rterm), bt2 = pk(bt, bt);
       const float one = exp2f(p.shift);
       uint64_t acc2 = 0;
       for (int i = 0; i < cnt; ++i, sr.next(), cr.next()) {
@@ -1043,23 +1049,32 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         tmem_ld_wait(v);
         float f[QC];
         const ulonglong2 *cq = reinterpret_cast<const ulonglong2 *>(col);
-#pragma unroll
-        for (int q = 0; q < QC / 4; ++q) {
-          const ulonglong2 bb = cq[q];
-          upk(add2(fma2(pk(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1])), l2e2, bb.x),
-                   rt2),
-              f[4 * q], f[4 * q + 1]);
-          upk(add2(fma2(pk(__uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3])), l2e2, bb.y),
-                   rt2),
-              f[4 * q + 2], f[4 * q + 3]);
-        }
-#pragma unroll
-        for (int q = 0; q < QC; ++q) f[q] = ex2(f[q]);
+        auto pair = [&](int q) {
+          return pk(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
+        };
         if (dw) {
-          // columns whose target is among this warp's 32 classes
+          // column terms: -lse; targets among this warp's 32 classes?
           const int *ctg = reinterpret_cast<const int *>(col + 2 * C::CN);
           const int off = ctg[lane % QC] - (tile * kTile + quad * 32);
-          if (__any_sync(~0u, off >= 0 && off < 32)) {
+          const bool any = __any_sync(~0u, off >= 0 && off < 32);
+          if (any) {
+#pragma unroll
+            for (int q = 0; q < QC / 2; q += 2) {
+              const ulonglong2 c = cq[q / 2];
+              upk(mul2(add2(add2(pair(q), bt2), c.x), l2e2), f[2 * q], f[2 * q + 1]);
+              upk(mul2(add2(add2(pair(q + 1), bt2), c.y), l2e2), f[2 * q + 2], f[2 * q + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < QC / 2; q += 2) {
+              const ulonglong2 c = cq[q / 2];
+              upk(fma2(add2(pair(q), c.x), l2e2, rt2), f[2 * q], f[2 * q + 1]);
+              upk(fma2(add2(pair(q + 1), c.y), l2e2, rt2), f[2 * q + 2], f[2 * q + 3]);
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < QC; ++q) f[q] = ex2(f[q]);
+          if (any) {
 #pragma unroll
             for (int q = 0; q < QC; ++q)
               if (ctg[q] == row) f[q] -= 1.f;
@@ -1075,11 +1090,28 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             upk(c, f[4 * q + 2], f[4 * q + 3]);
           }
         } else {
+          // column terms: bias * log2(e) + log2 of P's scale
           const int at = tg - ((c0 + i) * C::CN + w4 * QC);
-          if (__any_sync(~0u, at >= 0 && at < QC)) {
+          const bool any = __any_sync(~0u, at >= 0 && at < QC);
+          float pt = 0.f;
+          if (any) {
 #pragma unroll
             for (int q = 0; q < QC; ++q)
-              if (at == q) f[q] -= one;
+              if (at == q) pt = __uint_as_float(v[q]);
+            pt = ex2(fmaf((pt + bt) + rterm, kLog2e, p.shift)) - one;
+          }
+#pragma unroll
+          for (int q = 0; q < QC / 2; q += 2) {
+            const ulonglong2 c = cq[q / 2];
+            upk(fma2(add2(pair(q), rt2), l2e2, c.x), f[2 * q], f[2 * q + 1]);
+            upk(fma2(add2(pair(q + 1), rt2), l2e2, c.y), f[2 * q + 2], f[2 * q + 3]);
+          }
+#pragma unroll
+          for (int q = 0; q < QC; ++q) f[q] = ex2(f[q]);
+          if (any) {
+#pragma unroll
+            for (int q = 0; q < QC; ++q)
+              if (at == q) f[q] = pt;
           }
         }
         uint32_t h[QC / 2];
@@ -1289,6 +1321,7 @@ int launch_place(const Workspace &ws, const void *targets, bool wide, int rows, 
   p.V = V;
   p.K = K;
   p.shift = dtype == TOCR_DTYPE_F16 ? (float)(1 << kShift) : 1.f;
+  p.shift2 = dtype == TOCR_DTYPE_F16 ? (float)kShift : 0.f;
   p.bias = bias;
   p.bias2 = ws.bias2;
   p.cnt = ws.cnt;
@@ -1361,9 +1394,12 @@ TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *
   if (rc) return rc;
   FwdParams p{};
   p.feat = static_cast<const uint8_t *>(d_feat);
+  p.bias = d_bias;
   p.bias2 = ws.bias2;
   p.hdr = ws.hdr;
   p.rowidx = ws.rowidx;
+  p.tgt = ws.tgt;
+  p.lt = ws.lt;
   p.part = ws.part;
   p.V = num_classes;
   p.K = K;
@@ -1379,9 +1415,8 @@ TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *
     default: rc = bf ? launch_fwd<4, true>(p, d_w, grid, st) : launch_fwd<4, false>(p, d_w, grid, st);
   }
   if (rc) return rc;
-  return launch_overlapped("ce_loss_kernel", bf ? ce_loss_kernel<true> : ce_loss_kernel<false>,
-                           tiles * (kTile / 8), 256, 0, st, p, static_cast<const uint8_t *>(d_w),
-                           d_bias, ws.tgt, grid, d_loss, d_lse);
+  return launch_overlapped("ce_loss_kernel", ce_loss_kernel, tiles * (kTile / 8), 256, 0, st, p, grid,
+                           d_loss, d_lse);
 }
 
 TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, const float *d_bias,
@@ -1414,6 +1449,7 @@ TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, cons
   BwdParams p{};
   p.w = static_cast<const uint8_t *>(d_w);
   p.xc = ws.xc;
+  p.bias = d_bias;
   p.bias2 = ws.bias2;
   p.hdr = ws.hdr;
   p.rowidx = ws.rowidx;
