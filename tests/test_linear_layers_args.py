@@ -23,7 +23,8 @@ def test_cross_entropy_refusals(tocr):
                 dict(V=0), dict(dtype=2), dict(dtype=7), dict(feat=None), dict(w=None),
                 dict(targets=None), dict(loss=None), dict(lse=None), dict(ws=None), dict(err=None),
                 dict(feat=C.c_void_p(264)), dict(w=C.c_void_p(258)), dict(ws=C.c_void_p(272)),
-                dict(n=16)):
+                dict(n=16), dict(targets=C.c_void_p(258)), dict(loss=C.c_void_p(257)),
+                dict(err=C.c_void_p(258))):
         assert ce(lib, **bad) == INVALID, bad
         assert tocr._lib.last_error()
     assert ce(lib, rows=0, feat=None, targets=None, ws=None) == 0
@@ -39,7 +40,8 @@ def test_cross_entropy_backward_refusals(tocr):
     lib = tocr.lib()
     for bad in (dict(K=12), dict(rows=-1), dict(V=0), dict(dtype=2), dict(feat=None), dict(w=None),
                 dict(targets=None), dict(lse=None), dict(g=None), dict(ws=None), dict(err=None),
-                dict(dfeat=C.c_void_p(264)), dict(dw=C.c_void_p(8)), dict(n=16)):
+                dict(dfeat=C.c_void_p(264)), dict(dw=C.c_void_p(8)), dict(n=16),
+                dict(g=C.c_void_p(258)), dict(lse=C.c_void_p(257)), dict(db=C.c_void_p(258))):
         assert ce_back(lib, **bad) == INVALID, bad
     assert ce_back(lib, dfeat=None, dw=None, db=None, feat=None, w=None) == 0
     assert ce_back(lib, rows=0, dw=None, db=None, feat=None, w=None) == 0
@@ -67,6 +69,7 @@ def test_linear_refusals(tocr):
                 dict(act=3), dict(act=-1), dict(xt=3), dict(yt=-1), dict(x=None), dict(wq=None),
                 dict(sw=None), dict(y=None), dict(err=None), dict(wq=C.c_void_p(264)),
                 dict(x=C.c_void_p(257)), dict(y=C.c_void_p(257)), dict(x=C.c_void_p(258), xt=2),
+                dict(sw=C.c_void_p(258)), dict(err=C.c_void_p(257)),
                 dict(ws=None, **many), dict(ws=C.c_void_p(272), **many), dict(n=16, **many)):
         assert linear(lib, **bad) == INVALID, bad
     assert linear(lib, rows=0, x=None, y=None) == 0

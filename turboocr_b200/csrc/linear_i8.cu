@@ -796,7 +796,8 @@ TOCR_API int tocr_quant_rows_i8(const void *d_x, int x_dtype, long long rows, in
   TOCR_REQUIRE(d_x && d_codes && d_scales, "tocr_quant_rows_i8: null pointer");
   TOCR_REQUIRE(aligned(d_x, x_dtype == TOCR_DTYPE_F32 ? 4 : 2),
                "tocr_quant_rows_i8: x must be aligned to its element");
-  TOCR_REQUIRE(aligned(d_codes, 16), "tocr_quant_rows_i8: the codes must be 16-byte aligned");
+  TOCR_REQUIRE(aligned(d_codes, 16) && aligned(d_scales, 4),
+               "tocr_quant_rows_i8: the codes must be 16-byte, the scales 4-byte aligned");
   return quant_rows(d_x, x_dtype, rows, K, static_cast<int8_t *>(d_codes), d_scales,
                     as_stream(stream));
 }
@@ -812,6 +813,8 @@ TOCR_API int tocr_linear_i8_codes(const void *d_xq, const float *d_sx, long long
                "tocr_linear_i8_codes: the codes must be 16-byte aligned");
   TOCR_REQUIRE(aligned(d_y, out_dtype == TOCR_DTYPE_F32 ? 4 : 2),
                "tocr_linear_i8_codes: y must be aligned to its element");
+  TOCR_REQUIRE(aligned(d_sx, 4) && aligned(d_sw, 4) && aligned(d_bias, 4) && aligned(d_err, 4),
+               "tocr_linear_i8_codes: scales, bias and the error word must be 4-byte aligned");
   return run_product(d_xq, d_wq, params(d_sx, rows, K, d_sw, d_bias, N, act, d_y, d_err), K,
                      out_dtype, as_stream(stream));
 }
@@ -835,6 +838,8 @@ TOCR_API int tocr_linear_i8(const void *d_x, int x_dtype, long long rows, int K,
   TOCR_REQUIRE(aligned(d_x, x_dtype == TOCR_DTYPE_F32 ? 4 : 2) &&
                    aligned(d_y, out_dtype == TOCR_DTYPE_F32 ? 4 : 2),
                "tocr_linear_i8: x and y must be aligned to their elements");
+  TOCR_REQUIRE(aligned(d_sw, 4) && aligned(d_bias, 4) && aligned(d_err, 4),
+               "tocr_linear_i8: scales, bias and the error word must be 4-byte aligned");
   cudaStream_t st = as_stream(stream);
   LinParams p = params(nullptr, rows, K, d_sw, d_bias, N, act, d_y, d_err);
   if (is_few(rows, K)) {

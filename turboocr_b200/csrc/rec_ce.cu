@@ -1155,7 +1155,7 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         if (!whole)
           p.bpart[(size_t)slot * kTile + r] = s;
         else if (p.dbias)
-          p.dbias[row] = s * scale;
+          p.dbias[row] = s * p.unscale * p.hdr->gmax;
       }
 #pragma unroll
       for (int a = 0; a < KA; ++a) {
@@ -1257,7 +1257,7 @@ ce_join_kernel(const BwdParams p, int cn, int KP, int grid) {
       float s = p.bpart[(size_t)(2 * c - 1) * kTile + r];
 #pragma unroll 4
       for (int d = c; d <= last; ++d) s += p.bpart[(size_t)2 * d * kTile + r];
-      p.dbias[tile * kTile + r] = s * (gmax * p.unscale);
+      p.dbias[tile * kTile + r] = s * p.unscale * gmax;
     }
 }
 
@@ -1383,6 +1383,9 @@ TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *
                "tocr_rec_head_ce: null pointer");
   TOCR_REQUIRE(aligned(d_feat, 16) && aligned(d_w, 16),
                "tocr_rec_head_ce: features and weights must be 16-byte aligned");
+  TOCR_REQUIRE(aligned(d_targets, targets_i64 ? 8 : 4) && aligned(d_bias, 4) && aligned(d_loss, 4) &&
+                   aligned(d_lse, 4) && aligned(d_err, 4),
+               "tocr_rec_head_ce: a pointer is not aligned to its element");
   TOCR_REQUIRE(aligned(d_workspace, 256) &&
                    workspace_bytes >= carve(nullptr, rows, K, num_classes, false).bytes,
                "tocr_rec_head_ce: the workspace must be 256-byte aligned and hold %zu bytes",
@@ -1436,7 +1439,11 @@ TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, cons
   TOCR_REQUIRE(aligned(d_feat, 16) && aligned(d_w, 16) && aligned(d_dfeat, 16) && aligned(d_dw, 16),
                "tocr_rec_head_ce_backward: features, weights and their gradients must be 16-byte "
                "aligned");
-  TOCR_REQUIRE(aligned(d_workspace, 256) && workspace_bytes >= carve(nullptr, rows, K, num_classes, true).bytes,
+  TOCR_REQUIRE(aligned(d_targets, targets_i64 ? 8 : 4) && aligned(d_bias, 4) && aligned(d_lse, 4) &&
+                   aligned(d_grad_loss, 4) && aligned(d_dbias, 4) && aligned(d_err, 4),
+               "tocr_rec_head_ce_backward: a pointer is not aligned to its element");
+  TOCR_REQUIRE(aligned(d_workspace, 256) &&
+                   workspace_bytes >= carve(nullptr, rows, K, num_classes, true).bytes,
                "tocr_rec_head_ce_backward: the workspace must be 256-byte aligned and hold %zu bytes",
                carve(nullptr, rows, K, num_classes, true).bytes);
   cudaStream_t st = as_stream(stream);
