@@ -116,8 +116,9 @@ __device__ __forceinline__ void store_part(uint8_t *g, long long ldb, const uint
 
 template <typename T, bool SMALLK>
 __global__ void __launch_bounds__(kThreads, 1)
-linear_i8_rows_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
-                 const LinParams p) {
+linear_i8_rows_kernel(const __grid_constant__ CUtensorMap xmap,
+                      const __grid_constant__ CUtensorMap wmap,
+                      const LinParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
