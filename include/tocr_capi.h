@@ -172,7 +172,8 @@ TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, cons
 /* Rows of INT8 codes with one fp32 scale each: of activations (a scale per
  * token) or of a weight matrix [N][K] (a scale per output channel; lay it out
  * once). The per-pixel / per-channel numerics of tocr_dwpw_block:
- *   scale = max(max_k |x[k]| / 127, 2^-126) rounded to fp32,
+ *   scale = max(max_k |x[k]| * (1 / 127), 2^-126), 1 / 127 and the product
+ *           rounded to fp32,
  *   code[k] = x[k] / scale to the nearest integer (ties to even).
  * A row that holds an infinity or a NaN gets the scale NaN and codes 0.
  * d_x [rows][K] of x_dtype (any TOCR_DTYPE_*, aligned to its element);

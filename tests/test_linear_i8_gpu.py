@@ -20,7 +20,8 @@ def quantized(x):
     fp32 numbers is a tie only where the exact one is: q + 1/2 and its
     neighbours in reach differ by far more than 2^-45."""
     x32 = x.float()
-    s = (x32.abs().amax(1).cpu().double() / 127).float().clamp_min(2.0 ** -126).to(x.device)
+    top = x32.abs().amax(1).cpu().double()
+    s = (top * torch.tensor(1 / 127).double()).float().clamp_min(2.0 ** -126).to(x.device)
     bad = ~torch.isfinite(x32).all(1)
     q = torch.round(x32.double() / s.double()[:, None])
     q[bad] = 0

@@ -1,6 +1,7 @@
 // INT8 linear layer with a scale per token (row of x) and per output channel:
 //
-//   s_m  = max(max_k |x_mk| / 127, 2^-126)            (fp32, rounded once)
+//   s_m  = max(max_k |x_mk| * (1 / 127), 2^-126)      (1 / 127 and the product
+//                                                      rounded to fp32)
 //   q_mk = x_mk / s_m rounded to the nearest integer  (ties to even)
 //   y_mn = act(s_m t_n sum_k q_mk w_nk + b_n)         (w_nk, t_n: the weights'
 //                                                      codes and scales, made
@@ -81,6 +82,11 @@ __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s, float i
                      __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
 
+// a row's scale, from its largest |x|
+__device__ __forceinline__ float scale_of(float big) {
+  return fmaxf(big * (1.f / 127.f), 1.17549435e-38f);
+}
+
 // largest |x| of a 16-byte vector, as the bits of the type (monotonic; an
 // infinity or a NaN beats every number)
 template <typename T>
@@ -154,7 +160,7 @@ quant_rows_kernel(const T *__restrict__ x, long long rows, int K, int pitch,
   if (!live) return;
   const float big = from_bits<T>(top);
   const bool finite = big < INFINITY;  // false for NaN too
-  const float s = finite ? fmaxf(big / 127.f, 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
+  const float s = finite ? scale_of(big) : __uint_as_float(0x7fc00000u);
   if (tid == 0) scale[row] = s;
   const float inv = 1.f / s;
   int8_t *qr = q + row * pitch;
@@ -645,7 +651,7 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap wmap, const FewParams q
       }
       const float big = __uint_as_float(__reduce_max_sync(~0u, top));
       const bool finite = big < INFINITY;
-      const float s = finite ? fmaxf(big / 127.f, 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
+      const float s = finite ? scale_of(big) : __uint_as_float(0x7fc00000u);
       const float inv = 1.f / s;
       if (lane == 0) sx[r] = s;
 #pragma unroll 4

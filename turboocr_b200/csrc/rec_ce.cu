@@ -31,7 +31,9 @@
 //
 // Numbers: S, the softmax statistics, D and db are fp32. P is rounded to the
 // inputs' type for the second product (one rounding of each G_ij, relative
-// 2^-11 in fp16 and 2^-8 in bf16); fp16 holds it scaled by 2^14, so that a
+// 2^-11 in fp16 and 2^-8 in bf16), or, for dW of up to 512 rows, where one G_ij
+// can make up a row of dW and its error a visible part of it, to the sum of two
+// such numbers; fp16 holds it scaled by 2^14, so that a
 // probability of 2^-28 is still a normal number, and for dW the row weights
 // enter divided by their largest, so that small weights do not underflow.
 // The outputs are rounded once more to their type.
@@ -69,6 +71,7 @@ constexpr int kMaxK = 256;
 constexpr long long kMaxRows = 1ll << 24;
 constexpr int kMaxGrid = 148;    // CTAs of a product kernel: one per SM
 constexpr int kShift = 14;       // fp16: log2 of the scale of P
+constexpr int kSplitRows = 512;  // rows up to which dW takes P as two numbers
 
 // ------------------------------------------------------------- workspace ----
 struct Header {
@@ -340,6 +343,12 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack16(uint32_t v) {
+  if (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
 // y = S * log2(e) + terms of 32 columns, in pairs
@@ -845,7 +854,8 @@ struct BwdLine {
   }
 };
 
-template <int KA, bool BF16>
+// SPLIT: P of dW as the sum of two 16-bit numbers
+template <int KA, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
               const BwdParams p) {
@@ -988,6 +998,13 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             const uint32_t pc = (16 * k / C::QC) * C::QC + (16 * k % C::QC) / 2;
             mma_f16_ts(tmem + C::TD, pa + pc, bd + ((2048 * k) >> 4), id2, i > 0 || k > 0 ? 1u : 0u);
           }
+          if (SPLIT && dw) {  // and the second part of P behind the first
+#pragma unroll
+            for (int k = 0; k < C::CN / 16; ++k) {
+              const uint32_t pc = (16 * k / C::QC) * C::QC + (16 * k % C::QC) / 2 + C::QC / 2;
+              mma_f16_ts(tmem + C::TD, pa + pc, bd + ((2048 * k) >> 4), id2, 1u);
+            }
+          }
           mma_commit(&b_empty[b2.i]);
           b2.next();
           s2.next();
@@ -1121,6 +1138,17 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
           tmem_st16(ts, h);
         else
           tmem_st8(ts, h);
+        if (SPLIT && dw) {
+#pragma unroll
+          for (int q = 0; q < QC / 2; ++q) {
+            const float2 r = unpack16<BF16>(h[q]);
+            h[q] = pack16<BF16>(f[2 * q] - r.x, f[2 * q + 1] - r.y);
+          }
+          if constexpr (QC == 32)
+            tmem_st16(ts + QC / 2, h);
+          else
+            tmem_st8(ts + QC / 2, h);
+        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -1282,7 +1310,7 @@ int launch_fwd(const FwdParams &p, const void *w, int grid, cudaStream_t st) {
                            p);
 }
 
-template <int KA, bool BF16>
+template <int KA, bool BF16, bool SPLIT>
 int launch_bwd(const BwdParams &p, int rows_pad, int grid, cudaStream_t st) {
   using C = BwdCfg<KA>;
   CUtensorMap wm, xm;
@@ -1292,14 +1320,24 @@ int launch_bwd(const BwdParams &p, int rows_pad, int grid, cudaStream_t st) {
   if (rc) return rc;
   rc = tma_map_rows(&xm, ty, 2, p.xc, p.K, rows_pad, 2ll * p.K, C::CN);
   if (rc) return rc;
-  rc = allow_dynamic_smem(reinterpret_cast<const void *>(ce_bwd_kernel<KA, BF16>), C::SMEM,
+  rc = allow_dynamic_smem(reinterpret_cast<const void *>(ce_bwd_kernel<KA, BF16, SPLIT>), C::SMEM,
                           "ce_bwd_kernel");
   if (rc) return rc;
-  rc = launch_overlapped("ce_bwd_kernel", ce_bwd_kernel<KA, BF16>, grid, kThreads, C::SMEM, st, wm,
+  rc = launch_overlapped("ce_bwd_kernel", ce_bwd_kernel<KA, BF16, SPLIT>, grid, kThreads, C::SMEM, st, wm,
                          xm, p);
   if (rc || grid == 1) return rc;
   return launch_overlapped("ce_join_kernel", ce_join_kernel<BF16>, dim3(grid - 1, 8), 256, 0, st, p,
                            C::CN, C::KP, grid);
+}
+
+template <int KA>
+int launch_bwd_ka(const BwdParams &p, bool bf, bool split, int rows_pad, int grid,
+                  cudaStream_t st) {
+  if (bf)
+    return split ? launch_bwd<KA, true, true>(p, rows_pad, grid, st)
+                 : launch_bwd<KA, true, false>(p, rows_pad, grid, st);
+  return split ? launch_bwd<KA, false, true>(p, rows_pad, grid, st)
+               : launch_bwd<KA, false, false>(p, rows_pad, grid, st);
 }
 
 template <bool BWD>
@@ -1482,12 +1520,12 @@ TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, cons
   // two steps at least: fewer pieces to join (175 x 64 x 5000: 80 CTAs and not 148)
   const int grid = grid_for(tiles_x * p.chunks_v + p.tiles_w * chunks_r, 2);
   const int rows_pad = (int)((rows + kTile - 1) / kTile * kTile + kTile);
-  const bool bf = dtype == TOCR_DTYPE_BF16;
+  const bool bf = dtype == TOCR_DTYPE_BF16, split = rows <= kSplitRows;
   switch (KA) {
-    case 1: return bf ? launch_bwd<1, true>(p, rows_pad, grid, st) : launch_bwd<1, false>(p, rows_pad, grid, st);
-    case 2: return bf ? launch_bwd<2, true>(p, rows_pad, grid, st) : launch_bwd<2, false>(p, rows_pad, grid, st);
-    case 3: return bf ? launch_bwd<3, true>(p, rows_pad, grid, st) : launch_bwd<3, false>(p, rows_pad, grid, st);
-    default: return bf ? launch_bwd<4, true>(p, rows_pad, grid, st) : launch_bwd<4, false>(p, rows_pad, grid, st);
+    case 1: return launch_bwd_ka<1>(p, bf, split, rows_pad, grid, st);
+    case 2: return launch_bwd_ka<2>(p, bf, split, rows_pad, grid, st);
+    case 3: return launch_bwd_ka<3>(p, bf, split, rows_pad, grid, st);
+    default: return launch_bwd_ka<4>(p, bf, split, rows_pad, grid, st);
   }
 }
 

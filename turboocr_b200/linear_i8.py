@@ -31,8 +31,8 @@ def pitch(K: int) -> int:
 
 def quantize_rows(x: torch.Tensor, *, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes int8 [rows, pitch(K)], scales fp32 [rows]) of x [rows, K] (fp16,
-    bf16 or fp32): scale = max(max|x| / 127, 2^-126), code = x / scale to the
-    nearest integer, ties to even; zeros behind K. A row with an infinity or a
+    bf16 or fp32): scale = max(max|x| * (1 / 127), 2^-126) in fp32, code = x /
+    scale to the nearest integer, ties to even; zeros behind K. A row with an infinity or a
     NaN gets the scale NaN and codes 0."""
     if x.dim() != 2:
         raise ValueError("x is [rows, K]")
