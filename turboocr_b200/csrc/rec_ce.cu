@@ -31,9 +31,10 @@
 //
 // Numbers: S, the softmax statistics, D and db are fp32. P is rounded to the
 // inputs' type for the second product (one rounding of each G_ij, relative
-// 2^-11 in fp16 and 2^-8 in bf16), or, for dW of up to 512 rows, where one G_ij
-// can make up a row of dW and its error a visible part of it, to the sum of two
-// such numbers; fp16 holds it scaled by 2^14, so that a
+// 2^-11 in fp16 and 2^-8 in bf16), or, for up to 512 rows, where one G_ij can
+// make up most of a row of dF or dW and its error shows, to the sum of two such
+// numbers (such calls are a matter of latency: 43 us either way at 175 x 64 x
+// 5000); fp16 holds it scaled by 2^14, so that a
 // probability of 2^-28 is still a normal number, and for dW the row weights
 // enter divided by their largest, so that small weights do not underflow.
 // The outputs are rounded once more to their type.
@@ -71,7 +72,7 @@ constexpr int kMaxK = 256;
 constexpr long long kMaxRows = 1ll << 24;
 constexpr int kMaxGrid = 148;    // CTAs of a product kernel: one per SM
 constexpr int kShift = 14;       // fp16: log2 of the scale of P
-constexpr int kSplitRows = 512;  // rows up to which dW takes P as two numbers
+constexpr int kSplitRows = 512;  // rows up to which P is the sum of two numbers
 
 // ------------------------------------------------------------- workspace ----
 struct Header {
@@ -854,7 +855,7 @@ struct BwdLine {
   }
 };
 
-// SPLIT: P of dW as the sum of two 16-bit numbers
+// SPLIT: P as the sum of two 16-bit numbers
 template <int KA, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
@@ -998,7 +999,7 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             const uint32_t pc = (16 * k / C::QC) * C::QC + (16 * k % C::QC) / 2;
             mma_f16_ts(tmem + C::TD, pa + pc, bd + ((2048 * k) >> 4), id2, i > 0 || k > 0 ? 1u : 0u);
           }
-          if (SPLIT && dw) {  // and the second part of P behind the first
+          if (SPLIT) {  // and the second part of P behind the first
 #pragma unroll
             for (int k = 0; k < C::CN / 16; ++k) {
               const uint32_t pc = (16 * k / C::QC) * C::QC + (16 * k % C::QC) / 2 + C::QC / 2;
@@ -1138,7 +1139,7 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
           tmem_st16(ts, h);
         else
           tmem_st8(ts, h);
-        if (SPLIT && dw) {
+        if (SPLIT) {
 #pragma unroll
           for (int q = 0; q < QC / 2; ++q) {
             const float2 r = unpack16<BF16>(h[q]);
