@@ -183,11 +183,11 @@ TOCR_API int tocr_quant_rows_i8(const void *d_x, int x_dtype, long long rows, in
                                 float *d_scales, void *stream);
 
 /* y[m][n] = act(sx[m] sw[n] sum_k xq[m][k] wq[n][k] + bias[n]) on codes and
- * scales as tocr_quant_rows_i8 lays them out (both pitches K rounded up to 16,
- * zeros behind K). The sum is exact; the rest is fp32 (the channel's scale
- * first: sum * sw has to fit), rounded once to out_dtype. d_bias fp32 [N] or NULL; act TOCR_ACT_*; d_y [rows][N] of
- * out_dtype, aligned to its element, any N; d_err as in
- * tocr_rec_head_ctc_f16. */
+ * scales as tocr_quant_rows_i8 lays them out (both pitches K rounded up to 16;
+ * what lies behind K is not read). The sum is exact; the rest is fp32 (the
+ * channel's scale first: sum * sw has to fit), rounded once to out_dtype. d_bias
+ * fp32 [N] or NULL; act TOCR_ACT_*; d_y [rows][N] of out_dtype, aligned to its
+ * element, any N; d_err as in tocr_rec_head_ctc_f16. */
 TOCR_API int tocr_linear_i8_codes(const void *d_xq, const float *d_sx, long long rows, int K,
                                   const void *d_wq, const float *d_sw, const float *d_bias, int N,
                                   int act, int out_dtype, void *d_y, int *d_err, void *stream);

@@ -179,6 +179,37 @@ def test_few_tokens_border(tocr, cuda):
         check(x, w, None, "relu", BF16, err)
 
 
+@pytest.mark.parametrize("rows,K,N", [(3, 17, 5), (300, 17, 40), (130, 256, 33), (130, 260, 200),
+                                      (2100, 41, 18385)])
+def test_codes_of_any_origin(tocr, cuda, rows, K, N):
+    """All of int8, the code -128 and its largest sums among them, and anything
+    behind K. With scales of 1 the sums come out exactly (K 128^2 < 2^24)."""
+    g = torch.Generator(device="cpu").manual_seed(rows + K + N)
+    P = linear_i8.pitch(K)
+    xq = torch.randint(-128, 128, (rows, P), generator=g, dtype=torch.int8)
+    wq = torch.randint(-128, 128, (N, P), generator=g, dtype=torch.int8)
+    xq[0], wq[0], wq[1] = -128, -128, 127
+    xq, wq = xq.to(cuda), wq.to(cuda)
+    one = torch.ones(max(rows, N), device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    y = linear_i8.linear_codes(xq, one[:rows], K, wq, one[:N], None, out_dtype=F32, err=err)
+    want = xq[:, :K].double() @ wq[:, :K].double().T
+    assert int(err) == 0
+    assert torch.equal(y.double(), want)
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_weights_with_anything_behind_their_features(tocr, cuda, rows):
+    g = torch.Generator(device="cpu").manual_seed(rows)
+    x = torch.randn(rows, 21, generator=g).to(cuda)
+    wq, ws = linear_i8.quantize_rows(torch.randn(50, 21, generator=g).to(cuda))
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    a = linear_i8.linear(x, wq, ws, err=err)
+    wq[:, 21:] = 99
+    assert torch.equal(a, linear_i8.linear(x, wq, ws, err=err))
+    assert int(err) == 0
+
+
 def test_empty_and_other_streams_and_graphs(tocr, cuda):
     err = torch.zeros(1, dtype=torch.int32, device=cuda)
     w = torch.randn(500, 200, device=cuda)

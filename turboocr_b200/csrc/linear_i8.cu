@@ -467,11 +467,11 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
 }
 
 template <typename T, bool SMALLK>
-int launch_product(const void *xq, const void *wq, LinParams p, int pitch, cudaStream_t st) {
+int launch_product(const void *xq, const void *wq, LinParams p, int K, int pitch, cudaStream_t st) {
   CUtensorMap xm, wm;
-  int rc = tma_map_rows(&xm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, pitch, p.rows, pitch, p.bt);
+  int rc = tma_map_rows(&xm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, K, p.rows, pitch, p.bt);
   if (rc) return rc;
-  rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, pitch, p.N, pitch, kBM);
+  rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, K, p.N, pitch, kBM);
   if (rc) return rc;
   p.stages = kRingBytes / (kStageA + p.bt * 128);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
@@ -500,8 +500,8 @@ int product(const void *xq, const void *wq, LinParams p, int K, int pitch, cudaS
     }
   }
   p.tiles = p.tiles_n * ((p.rows + p.bt - 1) / p.bt);
-  return K <= kSmallK ? launch_product<T, true>(xq, wq, p, pitch, st)
-                      : launch_product<T, false>(xq, wq, p, pitch, st);
+  return K <= kSmallK ? launch_product<T, true>(xq, wq, p, K, pitch, st)
+                      : launch_product<T, false>(xq, wq, p, K, pitch, st);
 }
 
 // ---------------------------------------------------------------- few tokens --
@@ -735,7 +735,7 @@ template <typename X, typename T>
 int launch_few(FewParams q, const void *wq, int pitch, cudaStream_t st) {
   LinParams &p = q.lin;
   CUtensorMap wm;
-  int rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, pitch, p.N, pitch, kBM);
+  int rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, q.K, p.N, pitch, kBM);
   if (rc) return rc;
   q.vec = q.K % 4 == 0 && aligned(q.x, 4 * sizeof(X));
   p.bt = (int)(p.rows + kUnit - 1) / kUnit * kUnit;

@@ -78,7 +78,7 @@ struct TileWalk {
   }
 };
 
-// An s32 pair as fp32. SMALL: |sum| < 2^22, so adding it to the bits of
+// An s32 pair as fp32. SMALL: |sum| <= 2^22, so adding it to the bits of
 // 1.5 * 2^23 converts it (full-rate instructions; the conversion instruction runs
 // at an eighth of their rate and would bound layers of small K).
 template <bool SMALL>
@@ -88,6 +88,6 @@ __device__ __forceinline__ uint64_t sums2(uint32_t a, uint32_t b) {
                      ptx::pk(-12582912.f, -12582912.f));
   return ptx::pk((float)(int)a, (float)(int)b);
 }
-constexpr int kSmallK = 260;  // 127^2 K < 2^22
+constexpr int kSmallK = 256;  // 128^2 K <= 2^22: any codes
 
 }  // namespace tocr::linear

@@ -351,11 +351,11 @@ linear_i8_rows_kernel(const __grid_constant__ CUtensorMap xmap,
 }
 
 template <typename T, bool SMALLK>
-int launch_product(const void *xq, const void *wq, const LinParams &p, int pitch, cudaStream_t st) {
+int launch_product(const void *xq, const void *wq, const LinParams &p, int K, int pitch, cudaStream_t st) {
   CUtensorMap xm, wm;
-  int rc = tma_map_rows(&xm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, pitch, p.rows, pitch, kBM);
+  int rc = tma_map_rows(&xm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, K, p.rows, pitch, kBM);
   if (rc) return rc;
-  rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, pitch, p.N, pitch, p.bt);
+  rc = tma_map_rows(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, wq, K, p.N, pitch, p.bt);
   if (rc) return rc;
   auto *kernel = linear_i8_rows_kernel<T, SMALLK>;
   rc = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), kSmem, "linear_i8_rows_kernel");
@@ -387,8 +387,8 @@ int product(const void *xq, const void *wq, LinParams p, int K, int pitch, cudaS
   }
   p.tiles_n = (p.N + p.bt - kOverlap - 1) / (p.bt - kOverlap);
   p.tiles = tm * p.tiles_n;
-  return K <= kSmallK ? launch_product<T, true>(xq, wq, p, pitch, st)
-                      : launch_product<T, false>(xq, wq, p, pitch, st);
+  return K <= kSmallK ? launch_product<T, true>(xq, wq, p, K, pitch, st)
+                      : launch_product<T, false>(xq, wq, p, K, pitch, st);
 }
 
 }  // namespace
