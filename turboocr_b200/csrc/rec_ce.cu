@@ -65,6 +65,7 @@ constexpr int kTmemCols = 512;
 constexpr int kPolyPairs = 2;    // of 16 pairs of exponentials, those not left to the special-function unit
 constexpr int kColSlots = 8;     // ring of the streamed rows' per-row terms
 constexpr int kRowBlock = 256;   // rows per block of the numbering kernels
+constexpr int kJoinThreads = 256;
 constexpr int kDirect = 4;       // blocks whose rows the placing kernel counts itself
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -1224,15 +1225,21 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
   }
 }
 
-// Sums the pieces of the tiles that a range border cut, in the order of the
-// CTAs, and rounds them as the main kernel rounds a whole tile. blockIdx.x:
-// border (CTA c > 0), y: a slice of the tile.
+// Sums the pieces of the tiles that range borders cut, in a fixed order, and
+// rounds them as the main kernel rounds a whole tile. blockIdx.x: border (CTA b >
+// 0). The blocks of all borders inside a tile share its elements, and where that
+// leaves a block fewer than its threads, groups of threads share the pieces: few
+// rows cut the one tile of dF into many pieces (80 x 128 x 18385: 73, the
+// backward pass takes 27 us; 62 where one border's blocks sum a tile, a thread
+// per element).
 template <bool BF16>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kJoinThreads)
 ce_join_kernel(const BwdParams p, int cn, int KP, int grid) {
-  __shared__ int s_tile, s_dw, s_last;
+  __shared__ int s_tile, s_dw, s_first, s_last;
+  __shared__ float4 s_sum[kJoinThreads];
   after_previous();
-  if (threadIdx.x == 0) {
+  const int tid = threadIdx.x;
+  if (tid == 0) {
     s_tile = -1;
     const BwdLine line(p.hdr, cn, p.chunks_v, p.want_x, p.tiles_w);
     const Cuts cuts(line.total, grid);
@@ -1242,11 +1249,11 @@ ce_join_kernel(const BwdParams p, int cn, int KP, int grid) {
       bool dw;
       int tile, chunk, nc;
       line.at(at, dw, tile, chunk, nc);
-      const long long t0 = at - chunk;  // first step of the tile
-      // the first border inside a tile handles that tile
-      if (chunk > 0 && cuts.at(c - 1) <= t0) {
+      if (chunk > 0) {  // inside a tile
+        const long long t0 = at - chunk;  // first step of the tile
         s_tile = tile;
         s_dw = dw;
+        s_first = cuts.owner(t0) + 1;
         s_last = cuts.owner(t0 + nc - 1);
       }
     }
@@ -1255,38 +1262,65 @@ ce_join_kernel(const BwdParams p, int cn, int KP, int grid) {
   const int tile = s_tile;
   if (tile < 0) return;
   const bool dw = s_dw;
-  const int c = blockIdx.x + 1, last = s_last;  // pieces: the tail of CTA c - 1, then c .. last
+  const int c = s_first, borders = s_last - c + 1;
+  // pieces: the tail of CTA c - 1, then c .. last
+  const int pieces = borders + 1;
+  auto slot = [&](int j) { return 2 * (c + j - 1) + (j == 0 ? 1 : 0); };
+  const int slices = borders * gridDim.y;
+  const int slice = (blockIdx.x + 1 - c) * gridDim.y + blockIdx.y;
   const int lim = min(kTile, (dw ? p.V : p.hdr->n) - tile * kTile);
-  const int q4 = KP / 4;
+  const int q4 = KP / 4, total = lim * q4;  // elements: four columns of a row
   const float gmax = p.hdr->gmax;
-  const int step = gridDim.y * blockDim.x;
-  const size_t ps = (size_t)kTile * KP;
-  if (!dw || p.dw)
-    for (int e = blockIdx.y * blockDim.x + threadIdx.x; e < lim * q4; e += step) {
+  if (!dw || p.dw) {
+    int groups = 1;
+    while (groups < 32 && 2 * groups <= pieces &&
+           slices * (kJoinThreads / (2 * groups)) >= total)
+      groups *= 2;
+    const int width = kJoinThreads / groups, group = tid / width, el = tid % width;
+    for (int e0 = slice * width; e0 < total; e0 += slices * width) {
+      const int e = e0 + el;
       const int r = e / q4, k = (e - r * q4) * 4;
-      if (k >= p.K) continue;
-      const float *src = p.dpart + (size_t)r * KP + k;
-      float4 s = *reinterpret_cast<const float4 *>(src + (size_t)(2 * c - 1) * ps);
+      const bool mine = e < total && k < p.K;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (mine) {
+        const float *src = p.dpart + (size_t)r * KP + k;
 #pragma unroll 8
-      for (int d = c; d <= last; ++d) {
-        const float4 v = *reinterpret_cast<const float4 *>(src + 2 * (size_t)d * ps);
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+        for (int j = group; j < pieces; j += groups) {
+          const float4 v = *reinterpret_cast<const float4 *>(src + (size_t)slot(j) * kTile * KP);
+          s.x += v.x;
+          s.y += v.y;
+          s.z += v.z;
+          s.w += v.w;
+        }
       }
+      if (groups > 1) {
+        __syncthreads();
+        s_sum[tid] = s;
+        __syncthreads();
+        if (group == 0)
+          for (int g = 1; g < groups; ++g) {
+            const float4 v = s_sum[g * width + el];
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+          }
+      }
+      if (!mine || group) continue;
       const int row = tile * kTile + r;
       const float sc = (dw ? gmax : p.gc[row]) * p.unscale;
       uint8_t *out = dw ? p.dw + (size_t)row * p.K * 2 : p.dfeat + (size_t)p.rowidx[row] * p.K * 2;
       *reinterpret_cast<uint2 *>(out + 2 * k) =
           make_uint2(pack16<BF16>(s.x * sc, s.y * sc), pack16<BF16>(s.z * sc, s.w * sc));
     }
-  if (dw && p.dbias && blockIdx.y == 0)
-    for (int r = threadIdx.x; r < lim; r += blockDim.x) {
-      float s = p.bpart[(size_t)(2 * c - 1) * kTile + r];
-#pragma unroll 4
-      for (int d = c; d <= last; ++d) s += p.bpart[(size_t)2 * d * kTile + r];
-      p.dbias[tile * kTile + r] = s * p.unscale * gmax;
+  }
+  if (dw && p.dbias)  // a warp per class
+    for (int r = slice * (kJoinThreads / 32) + tid / 32; r < lim; r += slices * (kJoinThreads / 32)) {
+      float s = 0.f;
+      for (int j = tid % 32; j < pieces; j += 32) s += p.bpart[(size_t)slot(j) * kTile + r];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+      if (tid % 32 == 0) p.dbias[tile * kTile + r] = s * p.unscale * gmax;
     }
 }
 
@@ -1327,7 +1361,7 @@ int launch_bwd(const BwdParams &p, int rows_pad, int grid, cudaStream_t st) {
   rc = launch_overlapped("ce_bwd_kernel", ce_bwd_kernel<KA, BF16, SPLIT>, grid, kThreads, C::SMEM, st, wm,
                          xm, p);
   if (rc || grid == 1) return rc;
-  return launch_overlapped("ce_join_kernel", ce_join_kernel<BF16>, dim3(grid - 1, 8), 256, 0, st, p,
+  return launch_overlapped("ce_join_kernel", ce_join_kernel<BF16>, dim3(grid - 1, 4), kJoinThreads, 0, st, p,
                            C::CN, C::KP, grid);
 }
 
