@@ -15,7 +15,8 @@
 // NaN gets the scale NaN, so its outputs are NaN instead of silently wrong.
 //
 // Quantiser: one pass over x from memory (a row's values stay in registers
-// between its maximum and its codes); bound by HBM.
+// between its maximum and its codes). 16384 x 4096 bf16: 44 us, 4.6 TB/s of
+// 6.4; bound by the loads in flight that the registers leave room for.
 //
 // Product: the output channels are the rows of the MMA (M 128, the lanes of
 // tensor memory) and the tokens its columns (N = BT, 16 to 256), so a thread of
@@ -27,7 +28,9 @@
 // warp 0 loads 128 x 128-byte tiles of the weight codes and BT x 128-byte tiles
 // of the token codes by TMA (128-byte swizzle) into a ring, one thread of warp 1
 // issues tcgen05.mma kind::i8 into one of two TMEM accumulators, and sixteen
-// warps run the epilogue of the other.
+// warps run the epilogue of the other. 16384 x 4096 x 4096 bf16: 180 us, 3.05 POP/s
+// (the tensor pipe is 77 % busy); with K 128 and 18384 channels the stores are
+// the bound (366 us for 40960 tokens in fp16, 4.1 TB/s as a plain fill).
 #include <cmath>
 
 #include "linear_i8.cuh"

@@ -4,13 +4,14 @@
 //
 // Stores that fill a sector in part take the memory more than twice as long: the
 // kernel of linear_i8.cu, which stores 64 bytes of a row straight from
-// registers, needs 386 us for 40960 x 18384 (a plain fill of as many bytes takes
-// 387 us) but 815 us for 40960 x 18385, 992 us in a row of calls. Here the
-// columns that a warp works on overlap by 16: whatever a row's offset, the warp
-// has all channels of the whole sectors that it writes, and only the ends of y's
-// rows are written in part. 627 us, 634 us in a row of calls; bound by the
-// instructions of the epilogue (323 us without its stores), which is why sector-
-// aligned and small outputs stay with the other kernel (466 us here at 18384).
+// registers, needs 366 us for 40960 x 128 x 18384 in fp16 (a plain fill of as
+// many bytes takes 385 us) but 833 us for 18385 channels, 861 us in a row of
+// calls. Here the columns that a warp works on overlap by 16: whatever a row's
+// offset, the warp has all channels of the whole sectors that it writes, and only
+// the ends of y's rows are written in part. 587 us, in a row of calls too. Bound
+// by the load/store pipe, which the staging through shared memory and the stores
+// share (418 us with the stores alone, about 320 without them); sector-aligned
+// and small outputs stay with the other kernel (580 us here for 18384).
 //
 // The tokens are the rows of the MMA (M 128) and the channels its columns, so
 // that a row's channels are all in one warp's lanes. The warps read the

@@ -455,6 +455,14 @@ __device__ __forceinline__ void drain_loads(uint64_t *full, const Ring<N> &at) {
 }
 
 // ------------------------------------------------------------- forward ------
+// 40960 x 128 x 18385 fp16: 292 us, 660 TFLOP/s. One exponential per logit sets the
+// floor (167 us at the special-function unit's rate; it is 53 % busy); what else
+// keeps the warps is shared memory, whose port carries the streamed rows in, the
+// MMA's reads of them and the bias terms that each warp reads (231 us without the
+// exponentials, 188 without the terms as well, 159 for the product alone). Two
+// groups of eight warps take every other chunk and three S buffers keep the MMA
+// ahead of them; 64-row chunks, 24 warps and other splits measured the same or
+// slower.
 template <int KA>
 struct FwdCfg {
   static constexpr int KP = 64 * KA;
@@ -796,6 +804,13 @@ ce_loss_kernel(const FwdParams p, int grid, float *loss, float *lse) {
 }
 
 // ------------------------------------------------------------- backward -----
+// 10240 x 128 x 18385 fp16, half of the rows padding: 115 us, 840 TFLOP/s; 16384 x
+// 256 x 65537 bf16: 1390 us, 1.43 PFLOP/s of the four products, near what the GPU
+// sustains under its power cap. Every chunk is a chain S -> P -> D through all
+// sixteen warps; two S buffers let the MMA work on one while the warps have the
+// other (tensor pipe 52 % busy at K 128, 62 % at K 256). Chunks of 128 rows where
+// tensor memory has room (K up to 128), of 64 else; smaller chunks with more
+// buffers and two groups of warps measured slower (130 and 154 us).
 template <int KA>
 struct BwdCfg {
   static constexpr int KP = 64 * KA;
