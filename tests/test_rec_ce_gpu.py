@@ -118,6 +118,16 @@ def check(a, cuda, **kw):
     near(run(*a, cuda, **kw), exact(*a))
 
 
+@pytest.mark.parametrize("want", ["all", "feat", "weight", "bias"])
+@pytest.mark.parametrize("rows,K,V", [(40, 256, 30000), (80, 128, 18385), (40000, 128, 100),
+                                      (20000, 200, 130), (700, 64, 9000)])
+def test_tiles_in_many_pieces(tocr, cuda, rows, K, V, want):
+    """Few rows or few classes: one tile is cut by most of the ranges' borders."""
+    a = make(rows, K, V, torch.bfloat16, rows + V, cuda, bias=True)
+    kw = {} if want == "all" else {f"need_{n}": n == want for n in ("feat", "weight", "bias")}
+    near(run(*a, cuda, **kw), exact(*a))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_padding_rows_cost_and_reach_nothing(tocr, cuda, dtype):
     """NaN and infinities in padding rows leave every output as it is with zeros
