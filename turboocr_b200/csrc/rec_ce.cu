@@ -970,8 +970,11 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
   } else if (warp == 1) {
     if (elect_one()) {
       constexpr uint32_t id1 = BF16 ? idesc_bf16(kTile, C::CN) : idesc_f16(kTile, C::CN);
-      constexpr uint32_t id2 =
-          (BF16 ? idesc_bf16(kTile, C::KP) : idesc_f16(kTile, C::KP)) | kIdescBMnMajor;
+      // neither product takes more than 8 features of padding: steps of 16 in the
+      // first, columns of D in the second (8191 x 200 x 18385 bf16: 235 us, 255 with
+      // 256 features; the forward pass, bound elsewhere, gains nothing by it)
+      const int kn = (p.K + 15) / 16 * 16;
+      const uint32_t id2 = (BF16 ? idesc_bf16(kTile, kn) : idesc_f16(kTile, kn)) | kIdescBMnMajor;
       const uint64_t kdesc = sw128_kmajor_desc(smem_u32(smem));
       const uint64_t mdesc = sw128_mnmajor_desc(smem_u32(smem), C::CN * 128);
       Ring<C::STAGES> b1, b2;  // chunks of the first and of the second product
@@ -986,8 +989,9 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         const uint32_t d = tmem + C::TS + s1.i * C::CN;
 #pragma unroll
         for (int k = 0; k < 4 * KA; ++k)
-          mma_f16_ts(d, tmem + C::TX + 8 * k, bd + (((k >> 2) * (C::CN * 128) + 32 * (k & 3)) >> 4),
-                     id1, k > 0 ? 1u : 0u);
+          if (k <= 4 * KA - 4 || 16 * k < p.K)
+            mma_f16_ts(d, tmem + C::TX + 8 * k,
+                       bd + (((k >> 2) * (C::CN * 128) + 32 * (k & 3)) >> 4), id1, k > 0 ? 1u : 0u);
         mma_commit(&s_full[s1.i]);
         b1.next();
         s1.next();
