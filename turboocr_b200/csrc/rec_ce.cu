@@ -1209,6 +1209,7 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
 #pragma unroll
       for (int a = 0; a < KA; ++a) {
         const int col = (w4 * KA + a) * 16;
+        if (col >= p.K) break;  // no such columns of D
         uint32_t v[16];
         tmem_ld16(tl + C::TD + col, v);
         tmem_ld_wait(v);
