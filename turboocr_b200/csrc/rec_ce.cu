@@ -735,6 +735,7 @@ ce_fwd_kernel(const __grid_constant__ CUtensorMap wmap, const FwdParams p) {
       cp[(ew >> 2) * 2 * kTile + kTile + r] = sum;
       ok = named_bar_and(1, kEpiThreads, ok);
       if (!ok) break;
+      tc_fence_after();  // the products that both groups waited for are done with the tile
       if ((ew >> 2) == 0) {
         float M = top;
 #pragma unroll
