@@ -405,3 +405,55 @@ def test_offsets_beyond_32_bits(tocr, cuda):
     ref = p.T @ x
     assert bool(((dw[rows_at].double() - ref).abs() <= 2e-3 * ref.abs() + 1e-7).all())
     assert int(err) == 0
+
+
+# ---- several chunks of classes per CTA: 4096 rows are 32 tiles, 18385 classes 144 chunks, so
+# that each of 148 CTAs has 31 steps, and a class in the 64th chunk is not the first that a warp
+# sees but in the few CTAs whose range begins there
+MANY, CLASSES, FAR = 4096, 18385, 8192
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("column", [0, 1, 2, 3, 4, 18, 31])
+def test_one_class_far_above_the_others(tocr, cuda, column, dtype):
+    """A class whose logit is 90 to 1000 above the rest, at columns of every
+    kind, behind the chunks in which the sums got their base."""
+    f, w, b, t, gl = make(MANY, 64, CLASSES, dtype, 101 + column, cuda, pad=0.1)
+    t = torch.where(t == FAR + column, torch.ones_like(t), t)
+    for above in (90.0, 100.0, 176.0, 200.0, 300.0, 400.0, 1000.0):
+        b2 = b.clone()
+        b2[FAR + column] = above
+        check((f, w, b2, t, gl), cuda)
+
+
+@pytest.mark.parametrize("other", [FAR, FAR + 3, FAR + 4])
+def test_classes_masked_by_a_large_finite_bias(tocr, cuda, other):
+    """All classes but two masked with -1e4; the two have equal logits, so the
+    loss of one as the target is log 2."""
+    f, w, b, t, gl = make(MANY, 64, CLASSES, torch.float16, 111, cuda)
+    w[other], w[9000] = 0, 0
+    b = torch.full_like(b, -1e4)
+    b[other], b[9000] = 0, 0
+    t = torch.full_like(t, 9000)
+    got = run(f, w, b, t, gl, cuda)
+    near(got, exact(f, w, b, t, gl))
+    assert float((got["loss"] - math.log(2)).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("kind", ["rising", "falling", "steps", "far below", "spread"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_logits_of_any_size_over_many_chunks(tocr, cuda, kind, dtype):
+    f, w, b, t, gl = make(MANY, 64, CLASSES, dtype, 121, cuda, pad=0.1)
+    at = torch.arange(CLASSES, device=cuda)
+    ramp = torch.linspace(-900, 900, CLASSES, device=cuda)
+    if kind == "rising":
+        b = b + ramp
+    elif kind == "falling":
+        b = b - ramp
+    elif kind == "steps":        # every 1000 classes another level, up and down
+        b = b + ((at // 1000 * 7) % 19 - 9).float() * 37
+    elif kind == "far below":
+        b = b - 5000
+    else:
+        f = (f.float() * 40).to(dtype)
+    check((f, w, b, t, gl), cuda)

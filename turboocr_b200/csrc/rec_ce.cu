@@ -377,13 +377,15 @@ __device__ __forceinline__ void take_out(uint32_t (&v)[32], int at, float &taken
 }
 // exp2 of a pair without the special-function unit: y = n + f, |f| <= 1/2, by
 // adding and taking off 1.5 * 2^23; exp2(f) by its Taylor polynomial in f ln 2
-// up to f^6 (the next term is 1.2e-7 at |f| = 1/2, half a step of the result);
-// n goes into the exponent. y below -126 counts as -126 (2^-126 instead of
-// less), y up to 127.
+// up to f^6 (the next term is 1.2e-7 at |f| = 1/2; 2.2e-7 of the result at most
+// with the roundings, ex2.approx has 2.4e-7); n goes into the exponent. y below
+// -126 counts as -126 (2^-126 instead of less) and y above 128 as 128, whose n is
+// the exponent of an infinity and whose f is 0: what passes fp32 is an infinity
+// here as it is from the special-function unit, so that the sums show it.
 __device__ __forceinline__ uint64_t ex2_poly(uint64_t y) {
   float a, b;
   upk(y, a, b);
-  y = pk(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  y = pk(fminf(fmaxf(a, -126.f), 128.f), fminf(fmaxf(b, -126.f), 128.f));
   const uint64_t t = add2(y, pk(12582912.f, 12582912.f));
   const uint64_t n = add2(t, pk(-12582912.f, -12582912.f));
   const uint64_t f = fma2(n, pk(-1.f, -1.f), y);
