@@ -457,3 +457,26 @@ def test_logits_of_any_size_over_many_chunks(tocr, cuda, kind, dtype):
     else:
         f = (f.float() * 40).to(dtype)
     check((f, w, b, t, gl), cuda)
+
+
+@pytest.mark.parametrize("rows,V,at", [(200, 700, 96), (MANY, CLASSES, FAR)])
+@pytest.mark.parametrize("column", [0, 1, 2, 3, 4, 18, 31])
+def test_nan_class_shows_in_every_loss(tocr, cuda, rows, V, at, column):
+    """A NaN in the weights or the bias of one class, whatever its column, is a
+    NaN in the logits and so in the loss and lse of all rows but padding; an
+    infinite bias leaves no finite loss either."""
+    f, w, b, t, gl = make(rows, 64, V, torch.bfloat16, 131, cuda, pad=0.2)
+    t = torch.where(t == at + column, torch.zeros_like(t), t)
+    keep = t >= 0
+    err = err_word(cuda)
+    w2, b2, b3 = w.clone(), b.clone(), b.clone()
+    w2[at + column, 5] = math.nan
+    b2[at + column] = math.nan
+    b3[at + column] = math.inf
+    for ww, bb in ((w2, b), (w, b2)):
+        loss, lse = rec_head.cross_entropy(f, ww, bb, t, err=err)
+        assert bool(torch.isnan(loss[keep]).all()) and bool(torch.isnan(lse[keep]).all())
+        assert bool((loss[~keep] == 0).all()) and bool((lse[~keep] == 0).all())
+    loss, lse = rec_head.cross_entropy(f, w, b3, t, err=err)
+    assert not bool(torch.isfinite(loss[keep]).any()) and not bool(torch.isfinite(lse[keep]).any())
+    assert int(err) == 0

@@ -375,17 +375,24 @@ __device__ __forceinline__ void take_out(uint32_t (&v)[32], int at, float &taken
       v[q] = 0xff800000u;
     }
 }
+// x within [-126, 128]; NaN for NaN
+__device__ __forceinline__ float ex2_range(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;\n min.NaN.f32 %0, %0, %3;" : "=&f"(y) : "f"(x), "f"(-126.f), "f"(128.f));
+  return y;
+}
 // exp2 of a pair without the special-function unit: y = n + f, |f| <= 1/2, by
 // adding and taking off 1.5 * 2^23; exp2(f) by its Taylor polynomial in f ln 2
 // up to f^6 (the next term is 1.2e-7 at |f| = 1/2; 2.2e-7 of the result at most
-// with the roundings, ex2.approx has 2.4e-7); n goes into the exponent. y below
-// -126 counts as -126 (2^-126 instead of less) and y above 128 as 128, whose n is
-// the exponent of an infinity and whose f is 0: what passes fp32 is an infinity
-// here as it is from the special-function unit, so that the sums show it.
+// with the roundings, ex2.approx has 2.4e-7); 2^n from the bits of its exponent. y
+// below -126 counts as -126 (2^-126 instead of less). From 127.5 on n is 128, whose
+// bits are those of an infinity, and y above 128 counts as 128: what is about to
+// pass fp32 is an infinity here, so that the sums show it. A NaN stays one: the
+// bounds keep it, and 2^n is a factor, not a sum with the bits of exp2(f).
 __device__ __forceinline__ uint64_t ex2_poly(uint64_t y) {
   float a, b;
   upk(y, a, b);
-  y = pk(fminf(fmaxf(a, -126.f), 128.f), fminf(fmaxf(b, -126.f), 128.f));
+  y = pk(ex2_range(a), ex2_range(b));
   const uint64_t t = add2(y, pk(12582912.f, 12582912.f));
   const uint64_t n = add2(t, pk(-12582912.f, -12582912.f));
   const uint64_t f = fma2(n, pk(-1.f, -1.f), y);
@@ -396,11 +403,10 @@ __device__ __forceinline__ uint64_t ex2_poly(uint64_t y) {
   r = fma2(r, f, pk(2.4022651e-1f, 2.4022651e-1f));
   r = fma2(r, f, pk(6.9314718e-1f, 6.9314718e-1f));
   r = fma2(r, f, pk(1.f, 1.f));
-  float r0, r1, t0, t1;
-  upk(r, r0, r1);
+  float t0, t1;
   upk(t, t0, t1);
-  return pk(__uint_as_float(__float_as_uint(r0) + (__float_as_uint(t0) << 23)),
-            __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23)));
+  return mul2(r, pk(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
+                    __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u)));
 }
 // adds exp2(y) (exp2(y - base), nb = -base twice) of 32 columns to four sums
 template <bool BASE>
