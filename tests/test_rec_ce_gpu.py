@@ -480,3 +480,31 @@ def test_nan_class_shows_in_every_loss(tocr, cuda, rows, V, at, column):
     loss, lse = rec_head.cross_entropy(f, w, b3, t, err=err)
     assert not bool(torch.isfinite(loss[keep]).any()) and not bool(torch.isfinite(lse[keep]).any())
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("K", [64, 200])
+@pytest.mark.parametrize("rows,kept", [(0, 0), (5, 5), (300, 300), (700, 200), (700, 513),
+                                       (1500, 1000), (1500, 1490)])
+def test_infinite_weights_meet_no_padding(tocr, cuda, rows, kept, K):
+    """Without a row that has a target every gradient is zero, whatever the
+    weights hold. A class whose logit is -inf for every row (features above zero,
+    an infinite weight below) has probability zero and a zero gradient, also
+    where the rows do not fill their last tile."""
+    f, w, b, t, gl = make(rows, K, 500, torch.float16, 141, cuda)
+    f = f.abs() + 0.25
+    t = torch.where(t == 77, torch.zeros_like(t), t)
+    t[kept:] = -1
+    w[77] = -math.inf
+    got = run(f, w, b, t, gl, cuda, need_feat=False)
+    assert bool((got["dweight"][77] == 0).all()) and float(got["dbias"][77]) == 0
+    w2 = w.clone()
+    w2[77] = 0
+    b2 = b.clone()
+    b2[77] = -math.inf
+    two = run(f, w2, b2, t, gl, cuda, need_feat=False)
+    for k in ("loss", "lse", "dweight", "dbias"):
+        assert torch.equal(got[k], two[k]), k
+    w[78], w[79, 3] = math.inf, math.nan
+    got = run(f, w, b, torch.full_like(t, -1), gl, cuda)
+    for k, v in got.items():
+        assert bool((v == 0).all()), k

@@ -94,7 +94,7 @@ struct Workspace {
   float *lt;       // [rows_pad] the target's logit
   float2 *part;    // [tiles + grid][128] (base, sum) of a range's piece of a tile
   // backward
-  uint8_t *xc;     // [rows_pad][K] the kept rows of F, zero behind the last
+  uint8_t *xc;     // [rows_pad][K] the kept rows of F; behind the last, copies of one
   float *nlse;     // [rows_pad] -lse (-inf behind the last)
   float *gc;       // [rows_pad] g
   float *gs;       // [rows_pad] g / gmax * 2^shift
@@ -201,37 +201,49 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
   __shared__ int swarp[kRowBlock / 32];
   __shared__ int s_off, s_total;
   __shared__ float s_gmax;
+  __shared__ int s_seen, s_src;     // last kept row (direct) or block with one before this block; a kept row
   __shared__ int s_dst[kRowBlock];  // place of each row of the block, -1: padding
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   release_next();
   if (!p.direct) after_previous();
   // kept rows before this block, and the largest weight of all
-  int before = 0;
+  int before = 0, seen = -1;
   float gm = 0.f;
   if (p.direct) {
     const int mine = blockIdx.x * kRowBlock, upto = BWD ? p.rows : mine;
 #pragma unroll 4
     for (int k = tid; k < upto; k += kRowBlock) {
       if (target_of(p.targets, p.wide, k, p.V) < 0) continue;
-      if (k < mine) ++before;
+      if (k < mine) {
+        ++before;
+        seen = k;
+      }
       if (BWD) gm = fmaxf(gm, fabsf(p.g[k]));
     }
   } else {
     for (int b = tid; b < (int)gridDim.x; b += kRowBlock) {
-      if (b < (int)blockIdx.x) before += p.cnt[b];
+      if (b < (int)blockIdx.x && p.cnt[b]) {
+        before += p.cnt[b];
+        seen = b;
+      }
       if (BWD) gm = fmaxf(gm, p.gblk[b]);
     }
   }
-  if (tid == 0) s_off = 0;
+  if (tid == 0) {
+    s_off = 0;
+    s_seen = s_src = -1;
+  }
   __syncthreads();
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     before += __shfl_xor_sync(~0u, before, o);
     gm = fmaxf(gm, __shfl_xor_sync(~0u, gm, o));
+    if (BWD) seen = max(seen, __shfl_xor_sync(~0u, seen, o));
   }
   __shared__ float sg[kRowBlock / 32];
   if (lane == 0) {
     atomicAdd(&s_off, before);  // integers: the order does not matter
+    if (BWD) atomicMax(&s_seen, seen);
     sg[warp] = gm;
   }
   const long long row0 = (long long)blockIdx.x * kRowBlock;
@@ -293,23 +305,32 @@ __global__ void __launch_bounds__(kRowBlock) ce_place_kernel(const PlaceParams p
   }
   if (BWD) {
     s_dst[tid] = dst;
+    if (last) {  // some kept row: the last one
+      if (t >= 0 && dst == n - 1) s_src = (int)i;
+      if (s_total == 0 && s_seen >= 0) {
+        const int r = p.direct ? s_seen : s_seen * kRowBlock + tid;
+        if (target_of(p.targets, p.wide, r, p.V) >= 0) atomicMax(&s_src, r);
+      }
+    }
     __syncthreads();
     const int q = p.K / 8;  // 16-byte pieces of a row
     const int here = (int)min((long long)kRowBlock, (long long)p.rows - row0);
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const int from = blockIdx.y * kRowBlock + tid, step = gridDim.y * kRowBlock;
-    for (int e = from; e < here * q; e += step) {
+    // Behind the last row, copies of a kept one: their P is exp(-inf) = 0, which
+    // rows of zeros would not be sure of (0 times an infinite weight is a NaN).
+    // Without a kept row, zeros, whose products are not used.
+    const int pad = last ? end - n : 0;
+    for (int e = from; e < (here + pad) * q; e += step) {
       const int r = e / q, c = e - r * q;
-      const int d = s_dst[r];
+      const int d = r < here ? s_dst[r] : n + r - here;
+      const long long src = r < here ? row0 + r : s_src;
       if (d >= 0)
         reinterpret_cast<uint4 *>(p.xc)[(size_t)d * q + c] =
-            __ldg(reinterpret_cast<const uint4 *>(p.feat) + (size_t)(row0 + r) * q + c);
+            src >= 0 ? __ldg(reinterpret_cast<const uint4 *>(p.feat) + (size_t)src * q + c) : zero;
       else if (p.dfeat)
-        reinterpret_cast<uint4 *>(p.dfeat)[(size_t)(row0 + r) * q + c] = zero;
+        reinterpret_cast<uint4 *>(p.dfeat)[(size_t)src * q + c] = zero;
     }
-    if (last)
-      for (int e = from; e < (end - n) * q; e += step)
-        reinterpret_cast<uint4 *>(p.xc)[(size_t)n * q + e] = zero;
   }
 }
 
@@ -864,7 +885,7 @@ struct BwdLine {
   __device__ BwdLine(const Header *h, int cn, int cv, int want_x, int tw) {
     n = h->n;
     chunks_v = cv;
-    chunks_r = max(1, (n + cn - 1) / cn);  // no rows: one chunk of zeros, so that dW is written
+    chunks_r = max(1, (n + cn - 1) / cn);  // no rows: one chunk, so that zeros are written
     tiles_x = want_x ? (n + kTile - 1) / kTile : 0;
     tiles_w = tw;
     its_x = (long long)tiles_x * chunks_v;
@@ -1209,7 +1230,8 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         }
       }
       if (dw && real && w4 == 0) {
-        const float s = (bs[r] + bs[kTile + r]) + (bs[2 * kTile + r] + bs[3 * kTile + r]);
+        const float s =
+            line.n ? (bs[r] + bs[kTile + r]) + (bs[2 * kTile + r] + bs[3 * kTile + r]) : 0.f;
         if (!whole)
           p.bpart[(size_t)slot * kTile + r] = s;
         else if (p.dbias)
@@ -1223,6 +1245,10 @@ ce_bwd_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         tmem_ld16(tl + C::TD + col, v);
         tmem_ld_wait(v);
         if (!real) continue;
+        if (line.n == 0) {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) v[q] = 0;
+        }
         if (whole) {
           if (out) {
             uint32_t h[8];
