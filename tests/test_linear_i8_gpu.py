@@ -252,3 +252,29 @@ def test_output_beyond_32_bits(tocr, cuda):
     assert torch.equal(y[-300:], linear_i8.linear(x[-300:].contiguous(), wq, ws, None,
                                                   err=err)[:, :18368])
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("rows,N", [(300, 640), (2100, 18385)])
+def test_one_workspace_for_call_after_call(tocr, cuda, rows, N):
+    """Calls in a row on one stream with the same scratch memory, whose scales and
+    codes the product reads while it may already have begun beside the quantiser:
+    each has the bits of a call by itself."""
+    K = 200
+    g = torch.Generator(device="cpu").manual_seed(rows)
+    xs = [(torch.randn(rows, K, generator=g) * 4.0 ** k).half().to(cuda) for k in range(3)]
+    wq, ws = linear_i8.quantize_rows((torch.randn(N, K, generator=g) / math.sqrt(K)).to(cuda))
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    want = [linear_i8.linear(x, wq, ws, err=err) for x in xs]
+    n = tocr.lib().tocr_linear_i8_workspace_bytes(rows, K)
+    buf = torch.zeros(n, dtype=torch.uint8, device=cuda)
+    got = [torch.empty_like(y) for y in want * 4]
+    torch.cuda.synchronize()
+    for k, y in enumerate(got):
+        assert tocr.lib().tocr_linear_i8(
+            xs[k % 3].data_ptr(), 0, rows, K, wq.data_ptr(), ws.data_ptr(), None, N, 0, 0,
+            y.data_ptr(), buf.data_ptr(), n, err.data_ptr(),
+            torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    for k, y in enumerate(got):
+        assert torch.equal(y, want[k % 3]), k
+    assert int(err) == 0

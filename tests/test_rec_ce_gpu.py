@@ -508,3 +508,30 @@ def test_infinite_weights_meet_no_padding(tocr, cuda, rows, kept, K):
     got = run(f, w, b, torch.full_like(t, -1), gl, cuda)
     for k, v in got.items():
         assert bool((v == 0).all()), k
+
+
+@pytest.mark.parametrize("rows", [200, 1500])
+def test_one_workspace_for_backward_after_backward(tocr, cuda, rows):
+    """Backward calls in a row on one stream with the same scratch memory, in which
+    one kernel lays out the rows that the next one reads: each has the bits of a
+    call by itself."""
+    K, V = 72, 3000
+    sets = [make(rows, K, V, torch.float16, s, cuda, pad=0.3) for s in (151, 152, 153)]
+    want = [run(*s, cuda) for s in sets]
+    err = err_word(cuda)
+    n = tocr.lib().tocr_rec_head_ce_workspace_bytes(rows, K, V, 1)
+    buf = torch.zeros(n, dtype=torch.uint8, device=cuda)
+    got = [(torch.empty_like(f), torch.empty_like(w), torch.empty_like(b))
+           for f, w, b, _, _ in sets * 4]
+    torch.cuda.synchronize()
+    for k, o in enumerate(got):
+        f, w, b, t, gl = sets[k % 3]
+        assert tocr.lib().tocr_rec_head_ce_backward(
+            f.data_ptr(), w.data_ptr(), b.data_ptr(), t.data_ptr(), 0, rows, K, V, 0,
+            want[k % 3]["lse"].data_ptr(), gl.data_ptr(), *(x.data_ptr() for x in o),
+            buf.data_ptr(), n, err.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    for k, o in enumerate(got):
+        for v, name in zip(o, ("dfeat", "dweight", "dbias")):
+            assert torch.equal(v, want[k % 3][name]), (k, name)
+    assert int(err) == 0

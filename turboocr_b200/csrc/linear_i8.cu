@@ -405,8 +405,9 @@ linear_i8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
           (long long)t.mi * p.bt + (g + 4 * (lane / kUnit)) * kUnit + lane % kUnit;
       nsw = n < p.N ? __ldg(p.sw + n) : 0.f;
       nb = n < p.N && p.bias ? __ldg(p.bias + n) : 0.f;
-      ns0 = m < p.rows ? __ldg(p.sx + m) : 0.f;
-      ns1 = m + 8 * kUnit < p.rows ? __ldg(p.sx + m + 8 * kUnit) : 0.f;
+      // not read-only loads: the quantiser may still write when this kernel begins
+      ns0 = m < p.rows ? p.sx[m] : 0.f;
+      ns1 = m + 8 * kUnit < p.rows ? p.sx[m + 8 * kUnit] : 0.f;
     };
     TileWalk ahead(p);
     if (!ahead.done()) prefetch(ahead);

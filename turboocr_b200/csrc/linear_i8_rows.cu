@@ -253,7 +253,7 @@ linear_i8_rows_kernel(const __grid_constant__ CUtensorMap xmap,
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const long long m = (long long)t.mi * kBM + quad * 32 + 8 * i + (lane >> 2);
-        nsx[i] = m < p.rows ? __ldg(p.sx + m) : 0.f;
+        nsx[i] = m < p.rows ? p.sx[m] : 0.f;  // see linear_i8.cu: no read-only load
       }
     };
     TileWalk ahead(p);

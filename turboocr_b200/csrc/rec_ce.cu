@@ -452,7 +452,8 @@ __device__ __forceinline__ float sum4(const uint64_t (&s)[4]) {
 
 // One warp's share of a stationary tile into tensor memory: lane = row, the
 // warp's quarter `w4` of the features (8 * KA columns of two features).
-// src: this lane's row, or null for a zero row.
+// src: this lane's row, or null for a zero row. Not read-only loads: the rows may
+// be those that the kernel before, which may still run when this one begins, writes.
 template <int KA>
 __device__ __forceinline__ void load_tile_tmem(uint32_t tx, const uint8_t *src, int K, int w4) {
 #pragma unroll
@@ -460,8 +461,8 @@ __device__ __forceinline__ void load_tile_tmem(uint32_t tx, const uint8_t *src, 
     const int col = (w4 * KA + a) * 8;  // 16 features
     uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
     if (src) {
-      if (2 * col < K) v0 = __ldg(reinterpret_cast<const uint4 *>(src + 4 * col));
-      if (2 * col + 8 < K) v1 = __ldg(reinterpret_cast<const uint4 *>(src + 4 * col + 16));
+      if (2 * col < K) v0 = *reinterpret_cast<const uint4 *>(src + 4 * col);
+      if (2 * col + 8 < K) v1 = *reinterpret_cast<const uint4 *>(src + 4 * col + 16);
     }
     const uint32_t r[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
     tmem_st8(tx + col, r);
