@@ -184,7 +184,8 @@ TOCR_API int tocr_quant_rows_i8(const void *d_x, int x_dtype, long long rows, in
 
 /* y[m][n] = act(sx[m] sw[n] sum_k xq[m][k] wq[n][k] + bias[n]) on codes and
  * scales as tocr_quant_rows_i8 lays them out (both pitches K rounded up to 16;
- * what lies behind K is not read). The sum is exact; the rest is fp32 (the
+ * what lies behind K is not read), or any int8 codes. K below 2^17, so that the
+ * sum of K products of -128 fits s32. The sum is exact; the rest is fp32 (the
  * channel's scale first: sum * sw has to fit), rounded once to out_dtype. d_bias
  * fp32 [N] or NULL; act TOCR_ACT_*; d_y [rows][N] of out_dtype, aligned to its
  * element, any N; d_err as in tocr_rec_head_ctc_f16. */

@@ -278,3 +278,20 @@ def test_one_workspace_for_call_after_call(tocr, cuda, rows, N):
     for k, y in enumerate(got):
         assert torch.equal(y, want[k % 3]), k
     assert int(err) == 0
+
+
+def test_longest_sums_of_any_codes(tocr, cuda):
+    """The largest sums, of either sign, at the longest rows of codes: exact to the
+    one rounding to fp32."""
+    K = (1 << 17) - 1
+    xq = torch.full((40, K + 1), -128, dtype=torch.int8, device=cuda)
+    wq = torch.full((6, K + 1), -128, dtype=torch.int8, device=cuda)
+    wq[1::2] = 127
+    xq[5, ::2] = 127
+    one = torch.ones(40, device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    y = linear_i8.linear_codes(xq, one, K, wq, one[:6].contiguous(), None, out_dtype=F32, err=err)
+    assert int(err) == 0
+    assert torch.equal(y, (xq[:, :K].double() @ wq[:, :K].double().T).float())
+    with pytest.raises(ValueError):
+        linear_i8.linear_codes(xq, one, K + 1, wq, one[:6].contiguous(), None, out_dtype=F32, err=err)

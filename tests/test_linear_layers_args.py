@@ -110,3 +110,13 @@ def test_tensors_refused():
     with pytest.raises(ValueError, match="x is"):
         linear_i8.linear(f[0], w, e, err=e)
     assert linear_i8.pitch(1) == 16 and linear_i8.pitch(16) == 16 and linear_i8.pitch(1001) == 1008
+
+
+def test_codes_whose_sum_could_pass_32_bits(tocr):
+    """128^2 * 2^17 is 2^31: one feature more than the sums of any codes have room for."""
+    c = tocr.lib().tocr_linear_i8_codes
+    assert c(P, P, 4, 1 << 17, P, P, None, 10, 0, 0, P, P, None) == INVALID
+    assert tocr._lib.last_error()
+    assert 128 ** 2 * ((1 << 17) - 1) < 1 << 31
+    assert c(None, None, 0, (1 << 17) - 1, P, P, None, 10, 0, 0, None, P, None) == 0
+    assert tocr.lib().tocr_linear_i8_workspace_bytes(100, 1 << 17) > 100 << 17

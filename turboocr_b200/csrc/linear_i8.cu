@@ -8,7 +8,8 @@
 //                                                      by the same quantiser)
 //
 // the numerics that tocr_dwpw_block uses per pixel, for the recognizer's
-// linear layers. The sum is exact in s32 (K up to 131072); the epilogue is
+// linear layers. The sum is exact in s32 (K up to
+// 131072, with codes of -128 on both sides one less); the epilogue is
 // fp32, the channel's scale first (weights are of ordinary size, so neither the
 // largest nor the least activations leave fp32's range on the way), and rounds
 // once to the output type. A row that holds an infinity or a
@@ -765,15 +766,18 @@ int few(const FewParams &q, const void *wq, int pitch, int out_dtype, cudaStream
 }
 
 constexpr long long kMaxRows = 1ll << 24;
-constexpr int kMaxK = 1 << 17;  // 127^2 K stays inside s32
+// Sums stay inside s32: 127 * 128 K where one side's codes are the quantiser's
+// (-127 to 127), 128^2 K where both are any codes.
+constexpr int kMaxK = 1 << 17, kMaxCodesK = kMaxK - 1;
 constexpr int kMaxN = 1 << 24;
 
 bool is_dtype(int d) {
   return d == TOCR_DTYPE_F16 || d == TOCR_DTYPE_BF16 || d == TOCR_DTYPE_F32;
 }
 
-int check_linear(const char *fn, long long rows, int K, int N, int act, int out_dtype) {
-  TOCR_REQUIRE(rows >= 0 && rows <= kMaxRows && K > 0 && K <= kMaxK && N > 0 && N <= kMaxN,
+int check_linear(const char *fn, long long rows, int K, int most_k, int N, int act,
+                 int out_dtype) {
+  TOCR_REQUIRE(rows >= 0 && rows <= kMaxRows && K > 0 && K <= most_k && N > 0 && N <= kMaxN,
                "%s: bad sizes rows=%lld K=%d N=%d", fn, rows, K, N);
   TOCR_REQUIRE(act == TOCR_ACT_NONE || act == TOCR_ACT_RELU || act == TOCR_ACT_HARDSWISH,
                "%s: unknown activation %d", fn, act);
@@ -838,7 +842,7 @@ TOCR_API int tocr_linear_i8_codes(const void *d_xq, const float *d_sx, long long
                                   const void *d_wq, const float *d_sw, const float *d_bias, int N,
                                   int act, int out_dtype, void *d_y, int *d_err, void *stream) {
   TOCR_ENTRY();
-  int rc = check_linear("tocr_linear_i8_codes", rows, K, N, act, out_dtype);
+  int rc = check_linear("tocr_linear_i8_codes", rows, K, kMaxCodesK, N, act, out_dtype);
   if (rc || rows == 0) return rc;
   TOCR_REQUIRE(d_xq && d_sx && d_wq && d_sw && d_y && d_err, "tocr_linear_i8_codes: null pointer");
   TOCR_REQUIRE(aligned(d_xq, 16) && aligned(d_wq, 16),
@@ -861,7 +865,7 @@ TOCR_API int tocr_linear_i8(const void *d_x, int x_dtype, long long rows, int K,
                             void *d_y, void *d_workspace, size_t workspace_bytes, int *d_err,
                             void *stream) {
   TOCR_ENTRY();
-  int rc = check_linear("tocr_linear_i8", rows, K, N, act, out_dtype);
+  int rc = check_linear("tocr_linear_i8", rows, K, kMaxK, N, act, out_dtype);
   if (rc) return rc;
   TOCR_REQUIRE(is_dtype(x_dtype), "tocr_linear_i8: unknown type %d", x_dtype);
   if (rows == 0) return TOCR_OK;

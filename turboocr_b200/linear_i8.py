@@ -98,7 +98,8 @@ def linear_codes(xq: torch.Tensor, sx: torch.Tensor, K: int, wq: torch.Tensor, w
                  bias: torch.Tensor | None = None, *, err: torch.Tensor, act: str = "none",
                  out_dtype: torch.dtype = torch.float16, stream=None) -> torch.Tensor:
     """linear() on rows that quantize_rows has quantised already (several layers
-    on the same activations quantise them once)."""
+    on the same activations quantise them once), or on any int8 codes. K below
+    2^17 (products of -128 fill the 32 bits of the sum there)."""
     if xq.dim() != 2 or wq.dim() != 2:
         raise ValueError("xq is [rows, pitch(K)], wq is [N, pitch(K)]")
     dev = xq.get_device()
