@@ -139,7 +139,8 @@ TOCR_API int tocr_rec_head_ctc_f16(const void *d_feat, int batch_size, int seq_l
  * d_feat [rows][K] and d_w [num_classes][K] row-major, both of `dtype`
  * (TOCR_DTYPE_F16 or TOCR_DTYPE_BF16), 16-byte aligned; K a multiple of 8, 8
  * to 256; d_bias fp32 [num_classes] or NULL (a -inf entry masks its class);
- * d_targets int32, or int64 where targets_i64 is non-zero; rows up to 2^24.
+ * d_targets int32, or int64 where targets_i64 is non-zero; rows and num_classes
+ * up to 2^24.
  * d_loss, d_lse fp32 [rows]. d_workspace: 256-byte aligned, of the size that
  * tocr_rec_head_ce_workspace_bytes gives (0: sizes out of range); it is
  * scratch of one call, so calls that may overlap need their own. d_err as in

@@ -120,3 +120,14 @@ def test_codes_whose_sum_could_pass_32_bits(tocr):
     assert 128 ** 2 * ((1 << 17) - 1) < 1 << 31
     assert c(None, None, 0, (1 << 17) - 1, P, P, None, 10, 0, 0, None, P, None) == 0
     assert tocr.lib().tocr_linear_i8_workspace_bytes(100, 1 << 17) > 100 << 17
+
+
+def test_more_classes_than_the_calls_take(tocr):
+    """The workspace function gives 0 for sizes that the calls refuse."""
+    lib = tocr.lib()
+    f = lib.tocr_rec_head_ce_workspace_bytes
+    most = 1 << 24
+    for back in (0, 1):
+        assert f(4, 64, most, back) > 0 and f(4, 64, most + 1, back) == 0
+        assert f(4, 64, (1 << 31) - 1, back) == 0
+    assert ce(lib, V=most + 1) == INVALID and ce_back(lib, V=most + 1) == INVALID

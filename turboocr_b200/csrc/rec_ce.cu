@@ -71,6 +71,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxK = 256;
 constexpr long long kMaxRows = 1ll << 24;
+constexpr int kMaxClasses = 1 << 24;
 constexpr int kMaxGrid = 148;    // CTAs of a product kernel: one per SM
 constexpr int kShift = 14;       // fp16: log2 of the scale of P
 constexpr int kSplitRows = 512;  // rows up to which P is the sum of two numbers
@@ -1478,7 +1479,7 @@ int launch_place(const Workspace &ws, const void *targets, bool wide, int rows, 
 }
 
 int check_sizes(const char *fn, long long rows, int K, int V, int dtype) {
-  TOCR_REQUIRE(rows >= 0 && rows <= kMaxRows && V > 0 && V <= (1 << 24),
+  TOCR_REQUIRE(rows >= 0 && rows <= kMaxRows && V > 0 && V <= kMaxClasses,
                "%s: bad sizes rows=%lld classes=%d", fn, rows, V);
   TOCR_REQUIRE(K >= 8 && K <= kMaxK && K % 8 == 0,
                "%s: K must be a multiple of 8 up to 256 (got %d)", fn, K);
@@ -1496,7 +1497,9 @@ extern "C" {
 
 TOCR_API size_t tocr_rec_head_ce_workspace_bytes(long long rows, int K, int num_classes,
                                                  int backward) {
-  if (rows < 0 || rows > kMaxRows || K < 8 || K > kMaxK || K % 8 || num_classes <= 0) return 0;
+  if (rows < 0 || rows > kMaxRows || K < 8 || K > kMaxK || K % 8 || num_classes <= 0 ||
+      num_classes > kMaxClasses)
+    return 0;
   return carve(nullptr, rows, K, num_classes, backward != 0).bytes;
 }
 
