@@ -131,3 +131,19 @@ def test_more_classes_than_the_calls_take(tocr):
         assert f(4, 64, most, back) > 0 and f(4, 64, most + 1, back) == 0
         assert f(4, 64, (1 << 31) - 1, back) == 0
     assert ce(lib, V=most + 1) == INVALID and ce_back(lib, V=most + 1) == INVALID
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_cross_entropy_of_tensors_that_require_grad(which):
+    """It builds no graph, so it says so; under no_grad, and detached, the call is
+    as any other (here it gets as far as the device check)."""
+    x = [torch.zeros(4, 64, dtype=torch.float16), torch.zeros(10, 64, dtype=torch.float16),
+         torch.zeros(10)]
+    t, e = torch.zeros(4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    x[which].requires_grad_()
+    with pytest.raises(ValueError, match="no graph"):
+        rec_head.cross_entropy(*x, t, err=e)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+        rec_head.cross_entropy(*x, t, err=e)
+    with pytest.raises(ValueError, match="CUDA device"):
+        rec_head.cross_entropy(*(y.detach() for y in x), t, err=e)

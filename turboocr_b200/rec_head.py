@@ -51,7 +51,12 @@ def cross_entropy(feat: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
     and weight [classes, K] fp16 or bf16, K a multiple of 8 up to 256, bias
     fp32 [classes] or None, targets int32 or int64 [rows]. A target outside
     [0, classes) marks padding: loss and lse 0, and the row's features are not
-    looked at."""
+    looked at. Not an autograd function: the gradient is cross_entropy_backward's,
+    and tensors that require grad are refused where grad mode is on."""
+    if torch.is_grad_enabled() and (feat.requires_grad or weight.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
+        raise ValueError("the loss would carry no graph: call cross_entropy under torch.no_grad() "
+                         "or on detached tensors, and cross_entropy_backward for the gradient")
     dev, rows, K, V, pe, args = _common(feat, weight, bias, targets, err)
 
     def launch(s):
