@@ -159,7 +159,9 @@ TOCR_API int tocr_rec_head_ce(const void *d_feat, const void *d_w, const float *
  *   dfeat = G W, dw = G^T feat, dbias[j] = sum_i G[i][j].
  * d_dfeat [rows][K] and d_dw [num_classes][K] of `dtype`, d_dbias fp32; each
  * may be NULL (not wanted). Outputs are overwritten, not added to; padding
- * rows get zero gradients and their g and lse are not used. The workspace is
+ * rows get zero gradients and their g and lse are not used. G enters the
+ * products as the sum of two numbers of `dtype` for up to 512 rows, as one
+ * (relative error 2^-11 in fp16, 2^-8 in bf16) for more. The workspace is
  * that of backward = 1. Outputs must not overlap inputs. */
 TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, const float *d_bias,
                                        const void *d_targets, int targets_i64, long long rows,
@@ -172,7 +174,8 @@ TOCR_API int tocr_rec_head_ce_backward(const void *d_feat, const void *d_w, cons
 
 /* Rows of INT8 codes with one fp32 scale each: of activations (a scale per
  * token) or of a weight matrix [N][K] (a scale per output channel; lay it out
- * once). The per-pixel / per-channel numerics of tocr_dwpw_block:
+ * once). Symmetric, as in tocr_dwpw_block, whose scales (a division by 127) and
+ * codes may differ from these in their last place:
  *   scale = max(max_k |x[k]| * (1 / 127), 2^-126), 1 / 127 and the product
  *           rounded to fp32,
  *   code[k] = x[k] / scale to the nearest integer (ties to even).

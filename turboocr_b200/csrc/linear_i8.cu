@@ -7,8 +7,11 @@
 //                                                      codes and scales, made
 //                                                      by the same quantiser)
 //
-// the numerics that tocr_dwpw_block uses per pixel, for the recognizer's
-// linear layers. The sum is exact in s32 (K up to
+// for the recognizer's linear layers: symmetric codes and the two kinds of scales
+// as in tocr_dwpw_block, but not its bits. That block and its packer divide the
+// maximum by 127, which differs in the last place from the product here in one
+// row of 22, and the block's codes are products with 127 / max instead of exact
+// quotients by the scale. The sum is exact in s32 (K up to
 // 131072, with codes of -128 on both sides one less); the epilogue is
 // fp32, the channel's scale first (weights are of ordinary size, so neither the
 // largest nor the least activations leave fp32's range on the way), and rounds
@@ -512,9 +515,13 @@ int product(const void *xq, const void *wq, LinParams p, int K, int pitch, cudaS
 // ---------------------------------------------------------------- few tokens --
 // The same product for few tokens, whose quantiser is part of it: every CTA
 // makes the codes of all of them itself, in the layout of the MMA operand, while
-// its first weights arrive. Up to 32768 elements of x that takes under a
-// microsecond, less than a launch of its own (80 x 128 x 384 and 1 x 512 x 18385:
-// one launch and no scratch memory instead of two and some).
+// its first weights arrive: one launch and no scratch memory. That serves calls
+// that the host paces; on the device the rows that a warp takes one after the
+// other cost more than a second launch. us per call from Python, and replayed
+// from a graph, with the two launches behind the stroke: 1 x 512 x 18385 fp16
+// 11.4 / 16.1, 6.2 / 6.2; 80 x 128 x 384 11.3 / 15.8, 8.2 / 6.2; 128 x 256 x 1024
+// 14.4 / 16.0, 14.3 / 7.7; 8 x 4096 x 4096, where the rows are longest for the
+// limit, 18.5 / 16.0, 18.4 / 10.3.
 constexpr int kFewTokens = 128, kFewElements = 32768, kFewCodes = 64 * 1024, kFewStages = 8;
 
 bool is_few(long long rows, int K) {

@@ -1,6 +1,5 @@
 """INT8 linear layers with a scale per token and per output channel over the
-C-ABI: the numerics of the backbone's INT8 blocks for the recognizer's linear
-layers.
+C-ABI, for the recognizer's linear layers.
 
     wq, ws = linear_i8.quantize_rows(weight)          # [N, K], once
     y = linear_i8.linear(x, wq, ws, bias, act="hardswish", err=err)
