@@ -463,16 +463,21 @@ __device__ __forceinline__ float sum4(const uint64_t (&s)[4]) {
 // be those that the kernel before, which may still run when this one begins, writes.
 template <int KA>
 __device__ __forceinline__ void load_tile_tmem(uint32_t tx, const uint8_t *src, int K, int w4) {
+  uint4 v[KA][2];  // all loads first: they do not pass the stores
 #pragma unroll
   for (int a = 0; a < KA; ++a) {
     const int col = (w4 * KA + a) * 8;  // 16 features
-    uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
+    v[a][0] = v[a][1] = make_uint4(0, 0, 0, 0);
     if (src) {
-      if (2 * col < K) v0 = *reinterpret_cast<const uint4 *>(src + 4 * col);
-      if (2 * col + 8 < K) v1 = *reinterpret_cast<const uint4 *>(src + 4 * col + 16);
+      if (2 * col < K) v[a][0] = *reinterpret_cast<const uint4 *>(src + 4 * col);
+      if (2 * col + 8 < K) v[a][1] = *reinterpret_cast<const uint4 *>(src + 4 * col + 16);
     }
+  }
+#pragma unroll
+  for (int a = 0; a < KA; ++a) {
+    const uint4 &v0 = v[a][0], &v1 = v[a][1];
     const uint32_t r[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-    tmem_st8(tx + col, r);
+    tmem_st8(tx + (w4 * KA + a) * 8, r);
   }
 }
 
